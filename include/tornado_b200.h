@@ -91,7 +91,8 @@ enum tb200_prepare_class {
     TB200_PREPARE_GEMM_F32 = 4,
     TB200_PREPARE_GEMM_F16 = 8,
     TB200_PREPARE_PEER = 16,
-    TB200_PREPARE_ALL = 31
+    TB200_PREPARE_LAYER = 32, /* rmsnorm_quant, paged_plan, rope_append, paged_attention */
+    TB200_PREPARE_ALL = 63
 };
 int tb200_prepare(int op_classes);
 
@@ -407,6 +408,84 @@ int tb200_igemm_s32(int m, int n, int k, const int8_t *a, const int8_t *b, int32
 enum tb200_fp8_format { TB200_FP8_E4M3 = 0, TB200_FP8_E5M2 = 1 };
 int tb200_fp8gemm_f32(int m, int n, int k, int format, const uint8_t *a, const uint8_t *b, float *c, void *workspace,
                       size_t workspace_bytes, tb200_stream_t stream);
+
+/* ---- decoder layer: what lies between its quantised products -----------------------
+ * The norm whose 8-bit rows feed tb200_igemm_s32 / tb200_fp8gemm_f32 (or, with groups of 32, the mat-vecs'
+ * int8 blocks), the tables of a paged cache of keys and values, the write into it, and the attention that reads it.
+ * No counterpart in the reference, whose models write these as JIT kernels.  All arrays are device arrays of the
+ * calling thread's current CUDA context.  Pointers need the alignment of their element; 8 bytes (a payload behind
+ * either array header) keeps vector loads, 16 bytes the widest ones. */
+enum tb200_type { TB200_TYPE_F32 = 0, TB200_TYPE_F16 = 1, TB200_TYPE_BF16 = 2 }; /* the values of tb200_gemm_out */
+enum tb200_quant_format { TB200_Q_INT8 = 0, TB200_Q_E4M3 = 1, TB200_Q_E5M2 = 2 };
+
+/*   h = x + residual;  residual_out = h;  y = h / sqrt(mean(h * h) + eps) * weight;  q * scale = y
+ * x [rows] rows of `cols` elements of `type`, x_stride elements apart (>= cols); residual and residual_out [rows][cols]
+ * of the same type, each may be NULL (nothing is added / stored), and residual_out may be residual, or x when
+ * x_stride == cols; weight [cols] fp32.  The sum, the norm and the quantisation are fp32: y is that of the sum before
+ * residual_out's rounding.  q [rows][cols] holds int8, e4m3 or e5m2 (format) with one fp32 scale per `group` columns
+ * (32, 64, 128; the last group of a row may be shorter) in scales [rows][ceil(cols / group)], or one per row (group 0).
+ *   scale = max |y| / 127, 448 or 57344 of the group, 1 for a group of zeros;
+ *   int8: floor(y / scale + 1/2), the rule of tb200_quantize_x; fp8: to the nearest, ties to even.
+ * A group that holds an infinity or a NaN gets that as its scale and zeros as its values, so that the values it stands
+ * for are NaN. */
+int tb200_rmsnorm_quant(int rows, int cols, int type, const void *x, long long x_stride, const void *residual, void *residual_out,
+                        const float *weight, float eps, int format, int group, uint8_t *q, float *scales, tb200_stream_t stream);
+
+/* Lays out a step: request r has cached_lens[r] tokens in the cache and adds new_lens[r] (negative lengths count as 0).
+ * block_table [requests][max_pages] names the pages of each request; the ceil(cached / page_size) entries it holds
+ * stay, and the entries of the pages that the new tokens need are taken from free_pages [num_free] in order of
+ * requests.  Written besides:
+ *   cu_new [requests + 1]   first token row of each request in the step; the last entry is the number of rows used
+ *   kv_lens [requests]      cached + new
+ *   positions [max_tokens]  position of each token row in its request, -1 behind the last one
+ *   slots [max_tokens]      page * page_size + offset where the row's key and value belong, -1 behind the last row
+ *   counts [4]              rows laid out, rows asked for, pages taken, pages needed
+ * A request gets only the new tokens that its table row (max_pages * page_size positions) and the max_tokens rows
+ * hold: cu_new and kv_lens say how many, counts[0] < counts[1] says that some did not fit.  When free_pages runs out
+ * (counts[2] < counts[3]) the entries of the missing pages and the slots of their tokens are -1.  Entries that the step
+ * does not add are left as they were.  requests <= 16384, max_tokens <= 2^30, max_pages * page_size <= 2^30. */
+int tb200_paged_plan(int requests, int page_size, int max_pages, int max_tokens, int num_free, const int32_t *cached_lens,
+                     const int32_t *new_lens, const int32_t *free_pages, int32_t *block_table, int32_t *cu_new, int32_t *kv_lens,
+                     int32_t *positions, int64_t *slots, int32_t *counts, tb200_stream_t stream);
+
+/* Rotates the queries and keys of `tokens` rows by their positions and writes keys and values to their slots of the cache.
+ * q, k, v: rows of q_heads, kv_heads and kv_heads heads of head_dim elements of in_type; the rows of an array are
+ * q_stride, k_stride, v_stride elements apart (three parts of one fused projection, or arrays of their own); q_heads
+ * may be 0, with q and q_out NULL.  The first rot_dim (even, <= head_dim, may be 0) elements of a head are rotated in pairs
+ *   (a, b) -> (a cos - b sin, a sin + b cos)
+ * with cos_table, sin_table [table_rows][rot_dim / 2] fp32 at the row's position; pairs are (i, i + rot_dim / 2), or
+ * (2i, 2i + 1) when `interleaved`.  Results are rounded once to cache_type (F16 or BF16): q_out [tokens][q_heads][head_dim]
+ * (may be q itself where it has that type and layout), k_cache and v_cache [num_pages][kv_heads][page_size][head_dim].
+ * A row whose position is negative is left out altogether; one whose slot lies outside the cache gets its q_out and no
+ * place in the cache.  A position at or above table_rows leaves the row out as well and records TB200_ERR_INVALID_ARG
+ * (tb200_device_status).  Rows must not share a slot. */
+int tb200_rope_append(int tokens, int q_heads, int kv_heads, int head_dim, int in_type, const void *q, const void *k, const void *v,
+                      long long q_stride, long long k_stride, long long v_stride, const float *cos_table, const float *sin_table,
+                      int table_rows, int rot_dim, int interleaved, const int32_t *positions, int cache_type, void *q_out,
+                      int page_size, int num_pages, const int64_t *slots, void *k_cache, void *v_cache, tb200_stream_t stream);
+
+/* Attention of each request's new tokens over its cache, the new tokens' keys and values included:
+ *   out[i][h] = sum_j p_j V[j],  p = softmax over the visible j of scale * q[i][h] . K[j]
+ * q [tokens] rows of q_heads heads of head_dim, q_stride elements apart; the rows of request r are cu_new[r] ..
+ * cu_new[r + 1] - 1 (ascending; rows at or above `tokens` are not touched), query head h reads kv head
+ * h / (q_heads / kv_heads), and row i stands at position p = kv_lens[r] - rows of r + i.  Key j of the request lies in
+ * page block_table[r][j / page_size] (rows of max_pages entries) and is visible when 0 <= j <= p, j > p - window
+ * (window 0: no limit), j < max_pages * page_size, and its page is one of the cache's num_pages (others, -1 among
+ * them, count as masked).  A row that sees no key, or only scores of -infinity, gives zeros.  What the cache holds at
+ * places that a row does not see never reaches it, infinities and NaN included.
+ * q, out and the caches [num_pages][kv_heads][page_size][head_dim] are of one type, F16 or BF16; head_dim is a multiple
+ * of 8 up to 256, q_heads a multiple of kv_heads, scale > 0; the caches and out are 8-byte aligned.  out [tokens] rows
+ * of q_heads * head_dim elements, out_stride apart; rows behind the last request are left as they were.
+ * Scores, softmax and sums are fp32; probabilities are rounded to `type` for the product with V, and the result once.
+ * max_new: an upper bound on the rows of one request (0: unknown); it only chooses kernels and never changes what is
+ * computed.  The context of a request is split over the GPU and joined in a fixed order, so equal calls give equal
+ * results.  The workspace (16-byte aligned; tb200_paged_attention_workspace_bytes) needs no initialisation; two calls
+ * that can run at the same time need one each.  max_pages * page_size <= 2^30. */
+size_t tb200_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim);
+int tb200_paged_attention(int tokens, int requests, int max_new, int q_heads, int kv_heads, int head_dim, int type, const void *q,
+                          long long q_stride, const int32_t *cu_new, const int32_t *kv_lens, const int32_t *block_table, int max_pages,
+                          int page_size, int num_pages, const void *k_cache, const void *v_cache, float scale, int window, void *out,
+                          long long out_stride, void *workspace, size_t workspace_bytes, tb200_stream_t stream);
 
 #ifdef __cplusplus
 }

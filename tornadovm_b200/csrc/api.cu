@@ -33,6 +33,12 @@ int tu_status_read_async_hgemm(int *);
 int tu_status_clear_hgemm();
 int tu_status_read_async_peer(int *);
 int tu_status_clear_peer();
+int tu_status_read_async_rmsnorm(int *);
+int tu_status_clear_rmsnorm();
+int tu_status_read_async_paged_cache(int *);
+int tu_status_clear_paged_cache();
+int tu_status_read_async_attention(int *);
+int tu_status_clear_attention();
 
 
 // ---- options ---------------------------------------------------------------------------------
@@ -264,7 +270,10 @@ extern "C" int tb200_device_status_of(int op_classes, int *status_out) {
                                      {tu_status_read_async_gemv_tc, tu_status_clear_gemv_tc, TB200_PREPARE_GEMV_QUANT},
                                      {tu_status_read_async_sgemm, tu_status_clear_sgemm, TB200_PREPARE_GEMM_F32},
                                      {tu_status_read_async_hgemm, tu_status_clear_hgemm, TB200_PREPARE_GEMM_F16},
-                                     {tu_status_read_async_peer, tu_status_clear_peer, TB200_PREPARE_PEER}};
+                                     {tu_status_read_async_peer, tu_status_clear_peer, TB200_PREPARE_PEER},
+                                     {tu_status_read_async_rmsnorm, tu_status_clear_rmsnorm, TB200_PREPARE_LAYER},
+                                     {tu_status_read_async_paged_cache, tu_status_clear_paged_cache, TB200_PREPARE_LAYER},
+                                     {tu_status_read_async_attention, tu_status_clear_attention, TB200_PREPARE_LAYER}};
     constexpr int kReaders = sizeof(readers) / sizeof(readers[0]);
     // One word per translation unit: the reads are enqueued together into pinned memory and waited for once (a
     // host class calls this after every step; eight blocking copies cost more than the step's launch).

@@ -1,0 +1,232 @@
+// Paged attention: arguments, the division of the work over the blocks, and the joining of split rows.
+//
+// A call's work is a list of items (request, kv head, tile of query rows), each a run of key tiles.  The query rows of a
+// request for one kv head are its new tokens times the query heads that share the kv head, tokens first: row =
+// token * group + head of the group, so a decoding request has `group` rows and short chunks still fill a tile.  All
+// key tiles of all items, in order, are divided evenly over the grid: a block starts and ends inside an item, at most
+// two of its items are shared with neighbouring blocks, and every block has the same number of tiles whatever the
+// lengths are.  Lengths live on the device, so each block repeats the prefix sum over the requests by itself (reads
+// that L2 serves), and no block waits for another.
+//
+// A block that holds a whole item normalises and stores it.  Otherwise it leaves the running maximum, sum and
+// unnormalised output of its part in the workspace, in one of two places that belong to the block: 0 for an item that
+// an earlier block began, 1 for an item that it begins itself.  A second kernel joins the parts in the order of blocks.
+#pragma once
+
+#include "layer_common.cuh"
+
+namespace tb200 {
+
+struct AttnArgs {
+    const void *q, *k_cache, *v_cache;
+    const int32_t *cu_new, *kv_lens, *block_table;
+    void *out;
+    float *parts;        // [grid][2][rows of a tile][DPAD + 2 floats]: output, then maximum and sum
+    int4 *joins;         // [grid]: item that the block begins and another one ends: (request, kv head, row tile, last block), x < 0: none
+    long long q_stride, out_stride;
+    float scale_log2;    // scale * log2(e): probabilities are powers of two
+    int tokens, requests, q_heads, kv_heads, group, head_dim, max_pages, page_size, num_pages, window, page_shift;  // page_shift: log2, or -1
+    int min_rows, max_rows;  // only requests with min_rows <= rows <= max_rows are this kernel's
+};
+
+struct AttnRequest {
+    int first, rows, new_tokens;  // first token row; rows for one kv head; tokens in this step
+    int kv_len, visible;          // cached + new; keys that have a place in the table
+};
+
+// Lengths as they are used: whatever the arrays hold, nothing outside [0, tokens) and the table row is touched.
+__device__ __forceinline__ AttnRequest attn_request(const AttnArgs &a, int r) {
+    AttnRequest q;
+    const int b = min(max(a.cu_new[r], 0), a.tokens), e = min(max(a.cu_new[r + 1], b), a.tokens);
+    q.first = b, q.new_tokens = e - b;
+    const long long rows = (long long)q.new_tokens * a.group;
+    q.rows = rows >= a.min_rows && rows <= a.max_rows ? (int)rows : 0;
+    q.kv_len = min(max(a.kv_lens[r], 0), 1 << 30);
+    q.visible = (int)min((long long)q.kv_len, (long long)a.max_pages * a.page_size);
+    return q;
+}
+
+// Key tiles [first, first + count) that a tile of query rows sees; one (empty) tile where it sees none, so that every
+// row is written by somebody.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void attn_key_tiles(const AttnArgs &a, const AttnRequest &q, int tile, int &first, int &count) {
+    const int row0 = tile * ROWS, row1 = min(q.rows, row0 + ROWS) - 1;
+    const int base = q.kv_len - q.new_tokens;
+    const int lowest = base + row0 / a.group, highest = min(base + row1 / a.group, q.visible - 1);
+    first = a.window > 0 ? max(0, lowest - a.window + 1) / KEYS : 0;
+    const int last = highest < 0 ? -1 : highest / KEYS;
+    count = max(1, last - first + 1);
+}
+
+template <int ROWS, int KEYS>
+__device__ __forceinline__ long long attn_head_tiles(const AttnArgs &a, const AttnRequest &q) {
+    long long n = 0;
+    for (int t = 0; (long long)t * ROWS < q.rows; ++t) {
+        int first, count;
+        attn_key_tiles<ROWS, KEYS>(a, q, t, first, count);
+        n += count;
+    }
+    return n;
+}
+
+// First tile of block `b` of `blocks` over `total` tiles, and the block that has tile `u`.  blocks <= total: every block
+// between two that share an item has a part of it.
+__device__ __forceinline__ long long attn_block_begin(long long total, int b, int blocks) { return total / blocks * b + total % blocks * b / blocks; }
+__device__ __forceinline__ int attn_block_of(long long total, int blocks, long long u) {
+    int b = (int)min((long long)blocks - 1, u * blocks / total);  // exact up to rounding: step to the block that has it
+    while (b > 0 && attn_block_begin(total, b, blocks) > u) --b;
+    while (b + 1 < blocks && attn_block_begin(total, b + 1, blocks) <= u) ++b;
+    return b;
+}
+
+struct AttnStart {
+    long long total, begin, end;  // tiles of the call; this block's
+    int blocks;                   // blocks that have tiles
+    int request;                  // request in which the block begins
+    long long request_begin;      // first tile of that request
+};
+
+// Run by all threads of the block; `scan`: THREADS / 32 + 1 words of shared memory.
+template <int THREADS, int ROWS, int KEYS>
+__device__ __forceinline__ void attn_find_start(const AttnArgs &a, AttnStart *out, long long *scan) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (a.requests + THREADS - 1) / THREADS, r0 = min(a.requests, (int)threadIdx.x * per), r1 = min(a.requests, r0 + per);
+    long long mine = 0;
+    for (int r = r0; r < r1; ++r) mine += attn_head_tiles<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long w = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += w;
+    }
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    long long before = inc - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) before += scan[w];
+        total += scan[w];
+    }
+    const int blocks = (int)max(1LL, min((long long)gridDim.x, total)), b = blockIdx.x;
+    const long long begin = b < blocks ? attn_block_begin(total, b, blocks) : total, end = b < blocks ? attn_block_begin(total, b + 1, blocks) : total;
+    if (threadIdx.x == 0) out->total = total, out->begin = begin, out->end = end, out->blocks = blocks;
+    if (begin < end && before <= begin && begin < before + mine) {  // one thread
+        long long at = before;
+        int r = r0;
+        for (; r < r1; ++r) {
+            const long long n = attn_head_tiles<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
+            if (begin < at + n) break;
+            at += n;
+        }
+        out->request = r, out->request_begin = at;
+    }
+    __syncthreads();
+}
+
+// The block's walk over its items.
+template <int ROWS, int KEYS>
+struct AttnWalk {
+    AttnRequest q;
+    int request, head, tile;    // the item
+    int first, count;           // its key tiles
+    int from, to;               // this block's of them: [from, to) of [0, count)
+    long long item_begin;       // the item's first tile in the call
+
+    // The item that holds tile `at` of the call; `request` and `request_begin` (its first tile) are known.
+    __device__ __forceinline__ void seek(const AttnArgs &a, const AttnStart &s) {
+        request = s.request;
+        q = attn_request(a, request);
+        const long long per_head = attn_head_tiles<ROWS, KEYS>(a, q);
+        const long long in = s.begin - s.request_begin;
+        head = (int)(in / per_head);
+        item_begin = s.request_begin + head * per_head;
+        for (tile = 0;; ++tile) {
+            attn_key_tiles<ROWS, KEYS>(a, q, tile, first, count);
+            if (s.begin < item_begin + count) break;
+            item_begin += count;
+        }
+        clip(s);
+    }
+    __device__ __forceinline__ void clip(const AttnStart &s) {
+        from = (int)max(0LL, s.begin - item_begin);
+        to = (int)min((long long)count, s.end - item_begin);
+    }
+    // The next item; false when the block's tiles are done.
+    __device__ __forceinline__ bool next(const AttnArgs &a, const AttnStart &s) {
+        item_begin += count;
+        if (item_begin >= s.end) return false;
+        ++tile;
+        if ((long long)tile * ROWS >= q.rows) {
+            tile = 0;
+            if (++head >= a.kv_heads) {
+                head = 0;
+                do {
+                    q = attn_request(a, ++request);
+                } while (q.rows == 0);
+            }
+        }
+        attn_key_tiles<ROWS, KEYS>(a, q, tile, first, count);
+        clip(s);
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return from == 0 && to == count; }
+};
+
+// Joins the parts of the items that more than one block worked on.  Block x takes the item that block x of the main
+// kernel began and another one ended; the rows of the tile are spread over gridDim.y.  Each of the four warps takes
+// every fourth part; a lane holds DPAD / 32 columns.
+template <class T, int ROWS, int DPAD>
+__global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
+    constexpr int PITCH = DPAD + 2, COLS = DPAD / 32;
+    __shared__ float acc_s[4][DPAD], ml_s[4][2];
+    pdl_wait();
+    const int4 item = a.joins[blockIdx.x];
+    if (item.x < 0) return;
+    const AttnRequest q = attn_request(a, item.x);
+    const int rows = min(ROWS, q.rows - item.z * ROWS), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int parts = item.w - (int)blockIdx.x + 1;
+    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+        float m = -INFINITY, l = 0.0f, acc[COLS] = {};
+        for (int i = warp; i < parts; i += 4) {
+            const float *p = a.parts + (((long long)(blockIdx.x + i) * 2 + (i == 0)) * ROWS + row) * PITCH;
+            const float pm = p[DPAD], pl = p[DPAD + 1];
+            float v[COLS];
+#pragma unroll
+            for (int c = 0; c < COLS; c += 2) {
+                const float2 f = *reinterpret_cast<const float2 *>(p + lane * COLS + c);
+                v[c] = f.x, v[c + 1] = f.y;
+            }
+            if (pl == 0.0f) continue;  // a part that saw nothing
+            const float top = fmaxf(m, pm), w0 = exp2f(m - top), w1 = exp2f(pm - top);
+            l = l * w0 + pl * w1;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) acc[c] = acc[c] * w0 + v[c] * w1;
+            m = top;
+        }
+        __syncthreads();
+        if (lane == 0) ml_s[warp][0] = m, ml_s[warp][1] = l;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc_s[warp][lane * COLS + c] = acc[c];
+        __syncthreads();
+        float top = -INFINITY, sum = 0.0f, w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = ml_s[i][1] == 0.0f ? top : fmaxf(top, ml_s[i][0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = ml_s[i][1] == 0.0f ? 0.0f : exp2f(ml_s[i][0] - top);
+            sum += ml_s[i][1] * w[i];
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int at = item.z * ROWS + row, token = at / a.group, head = item.y * a.group + at % a.group;
+        T *dst = static_cast<T *>(a.out) + (q.first + token) * a.out_stride + (long long)head * a.head_dim;
+        for (int d = threadIdx.x; d < a.head_dim; d += 128) {
+            float v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (w[i] != 0.0f) v += acc_s[i][d] * w[i];
+            from_f32(dst[d], v * inv);
+        }
+    }
+}
+
+}  // namespace tb200

@@ -13,7 +13,7 @@ import os
 
 from .build import LIB_PATH
 
-_I, _P, _F, _Z = C.c_int, C.c_void_p, C.c_float, C.c_size_t
+_I, _P, _F, _Z, _L = C.c_int, C.c_void_p, C.c_float, C.c_size_t, C.c_longlong
 
 # name -> (restype, argtypes); mirrors include/tornado_b200.h one to one
 SIGNATURES = {
@@ -60,6 +60,11 @@ SIGNATURES = {
     "tb200_igemm_workspace_bytes": (_Z, [_I, _I]),
     "tb200_igemm_s32": (_I, [_I, _I, _I, _P, _P, _P, _P, _Z, _P]),
     "tb200_fp8gemm_f32": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _Z, _P]),
+    "tb200_rmsnorm_quant": (_I, [_I, _I, _I, _P, _L, _P, _P, _P, _F, _I, _I, _P, _P, _P]),
+    "tb200_paged_plan": (_I, [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "tb200_rope_append": (_I, [_I, _I, _I, _I, _I, _P, _P, _P, _L, _L, _L, _P, _P, _I, _I, _I, _P, _I, _P, _I, _I, _P, _P, _P, _P]),
+    "tb200_paged_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "tb200_paged_attention": (_I, [_I, _I, _I, _I, _I, _I, _I, _P, _L, _P, _P, _P, _I, _I, _I, _P, _P, _F, _I, _P, _L, _P, _Z, _P]),
     "tb200_hgemm_f32_scatter": (_I, [_I, _I, _I, _P, _P, _P, _I, C.c_longlong, C.c_longlong, _P]),
 }
 
