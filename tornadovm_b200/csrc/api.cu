@@ -39,6 +39,8 @@ int tu_status_read_async_paged_cache(int *);
 int tu_status_clear_paged_cache();
 int tu_status_read_async_attention(int *);
 int tu_status_clear_attention();
+int tu_status_read_async_attention_tc(int *);
+int tu_status_clear_attention_tc();
 
 
 // ---- options ---------------------------------------------------------------------------------
@@ -273,7 +275,8 @@ extern "C" int tb200_device_status_of(int op_classes, int *status_out) {
                                      {tu_status_read_async_peer, tu_status_clear_peer, TB200_PREPARE_PEER},
                                      {tu_status_read_async_rmsnorm, tu_status_clear_rmsnorm, TB200_PREPARE_LAYER},
                                      {tu_status_read_async_paged_cache, tu_status_clear_paged_cache, TB200_PREPARE_LAYER},
-                                     {tu_status_read_async_attention, tu_status_clear_attention, TB200_PREPARE_LAYER}};
+                                     {tu_status_read_async_attention, tu_status_clear_attention, TB200_PREPARE_LAYER},
+                                     {tu_status_read_async_attention_tc, tu_status_clear_attention_tc, TB200_PREPARE_LAYER}};
     constexpr int kReaders = sizeof(readers) / sizeof(readers[0]);
     // One word per translation unit: the reads are enqueued together into pinned memory and waited for once (a
     // host class calls this after every step; eight blocking copies cost more than the step's launch).
@@ -322,7 +325,7 @@ extern "C" int tb200_prepare(int op_classes) {
         st = prepare_kernel(e, di);
         if (st) return st;
     }
-    if (op_classes & TB200_PREPARE_GEMM_F16) {
+    if (op_classes & (TB200_PREPARE_GEMM_F16 | TB200_PREPARE_LAYER)) {
         st = hgemm_prepare_driver();
         if (st) return st;
     }

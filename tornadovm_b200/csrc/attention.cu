@@ -18,6 +18,7 @@ TB200_TU_STATUS(attention)
 namespace tb200 {
 
 constexpr int AT_THREADS = 128, AT_KEYS = 64;
+constexpr int AT_TC_ROWS = 64;   // requests of more rows go to the tensor-memory kernel
 constexpr int AT_MAX_SMS = 148;  // the workspace is sized without asking the device
 
 __device__ __forceinline__ float ex2(float x) {
@@ -453,7 +454,7 @@ static bool attn_shape_ok(int tokens, int requests, int q_heads, int kv_heads, i
 
 extern "C" size_t tb200_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim) {
     if (!attn_shape_ok(tokens, requests, q_heads, kv_heads, head_dim)) return 0;
-    return attn_any_workspace(head_dim);
+    return max(attn_any_workspace(head_dim), attn_tc_workspace(head_dim));
 }
 
 extern "C" int tb200_paged_attention(int tokens, int requests, int max_new, int q_heads, int kv_heads, int head_dim, int type, const void *q,
@@ -483,5 +484,7 @@ extern "C" int tb200_paged_attention(int tokens, int requests, int max_new, int 
     a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
     a.min_rows = 1, a.max_rows = 0x7FFFFFFF;
     const long long longest = (long long)(max_new > 0 ? min(max_new, tokens) : tokens) * a.group;
-    return attn_any_launch(a, type, (int)min(longest, 0x7FFFFFFFLL), workspace, di, (cudaStream_t)stream);
+    const int rows = (int)min(longest, 0x7FFFFFFFLL);
+    if (rows > AT_TC_ROWS && attn_tc_eligible(a)) return attn_tc_launch(a, type, rows, workspace, di, (cudaStream_t)stream);
+    return attn_any_launch(a, type, rows, workspace, di, (cudaStream_t)stream);
 }

@@ -229,4 +229,9 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
     }
 }
 
+// attention_tc.cu
+bool attn_tc_eligible(const AttnArgs &a);
+int attn_tc_launch(const AttnArgs &a, int type, int longest_rows, void *workspace, const DeviceInfo *di, cudaStream_t s);
+size_t attn_tc_workspace(int head_dim);
+
 }  // namespace tb200
