@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
     long long *row_s = reinterpret_cast<long long *>(kv_s + STAGES * 2 * TILE_BYTES);  // [RING][64]: row of the cache, -1: none
     int *hole_s = reinterpret_cast<int *>(row_s + RING * AT_KEYS);                     // [RING][2]: a row of the tile's half is missing
     __shared__ AttnStart start;
-    __shared__ long long scan[AT_THREADS / 32 + 1];
+    __shared__ long long scan[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int D = a.head_dim, ksteps = (D + 15) / 16, dchunks = D / 8, lchunks = 2 * ksteps;
     const int warp_key = SPLIT_KEYS ? warp * 16 : 0, warp_row = SPLIT_KEYS ? 0 : warp * 16;

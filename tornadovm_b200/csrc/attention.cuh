@@ -58,6 +58,7 @@ __device__ __forceinline__ void attn_key_tiles(const AttnArgs &a, const AttnRequ
     count = max(1, last - first + 1);
 }
 
+// Key tiles of all row tiles of a request for one head: by one thread, and by a warp.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ long long attn_head_tiles(const AttnArgs &a, const AttnRequest &q) {
     long long n = 0;
@@ -66,6 +67,18 @@ __device__ __forceinline__ long long attn_head_tiles(const AttnArgs &a, const At
         attn_key_tiles<ROWS, KEYS>(a, q, t, first, count);
         n += count;
     }
+    return n;
+}
+template <int ROWS, int KEYS>
+__device__ __forceinline__ long long attn_head_tiles_warp(const AttnArgs &a, const AttnRequest &q) {
+    long long n = 0;
+    for (int t = threadIdx.x & 31; (long long)t * ROWS < q.rows; t += 32) {
+        int first, count;
+        attn_key_tiles<ROWS, KEYS>(a, q, t, first, count);
+        n += count;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
 }
 
@@ -86,34 +99,51 @@ struct AttnStart {
     long long request_begin;      // first tile of that request
 };
 
-// Run by all threads of the block; `scan`: THREADS / 32 + 1 words of shared memory.
+// Run by all threads of the block; `scan`: 32 words of shared memory.  Few requests are counted by a warp each (a long
+// prompt has hundreds of row tiles), many by a thread each.
 template <int THREADS, int ROWS, int KEYS>
 __device__ __forceinline__ void attn_find_start(const AttnArgs &a, AttnStart *out, long long *scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = (a.requests + THREADS - 1) / THREADS, r0 = min(a.requests, (int)threadIdx.x * per), r1 = min(a.requests, r0 + per);
+    const bool few = a.requests <= 32;
     long long mine = 0;
-    for (int r = r0; r < r1; ++r) mine += attn_head_tiles<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
+    int r0 = 0, r1 = 0;
+    if (few) {
+        for (int r = warp; r < a.requests; r += THREADS / 32) {
+            const long long n = attn_head_tiles_warp<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
+            if (lane == 0) scan[r] = n;
+        }
+        __syncthreads();
+        mine = lane < a.requests ? scan[lane] : 0;  // every warp: a request per lane
+    } else {
+        const int per = (a.requests + THREADS - 1) / THREADS;
+        r0 = min(a.requests, (int)threadIdx.x * per), r1 = min(a.requests, r0 + per);
+        for (int r = r0; r < r1; ++r) mine += attn_head_tiles<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
+    }
     long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long w = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += w;
     }
-    if (lane == 31) scan[warp] = inc;
-    __syncthreads();
     long long before = inc - mine, total = 0;
+    if (few) {
+        total = __shfl_sync(0xffffffffu, inc, 31);
+    } else {
+        if (lane == 31) scan[warp] = inc;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) before += scan[w];
-        total += scan[w];
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) before += scan[w];
+            total += scan[w];
+        }
     }
     const int blocks = (int)max(1LL, min((long long)gridDim.x, total)), b = blockIdx.x;
     const long long begin = b < blocks ? attn_block_begin(total, b, blocks) : total, end = b < blocks ? attn_block_begin(total, b + 1, blocks) : total;
     if (threadIdx.x == 0) out->total = total, out->begin = begin, out->end = end, out->blocks = blocks;
-    if (begin < end && before <= begin && begin < before + mine) {  // one thread
+    if (begin < end && before <= begin && begin < before + mine && (warp == 0 || !few)) {  // one thread
         long long at = before;
-        int r = r0;
-        for (; r < r1; ++r) {
+        int r = few ? lane : r0;
+        for (; !few && r < r1; ++r) {
             const long long n = attn_head_tiles<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
             if (begin < at + n) break;
             at += n;
@@ -132,18 +162,32 @@ struct AttnWalk {
     int from, to;               // this block's of them: [from, to) of [0, count)
     long long item_begin;       // the item's first tile in the call
 
-    // The item that holds tile `at` of the call; `request` and `request_begin` (its first tile) are known.
+    // The item that holds the block's first tile; run by whole warps, whose lanes look at 32 row tiles at a time.
     __device__ __forceinline__ void seek(const AttnArgs &a, const AttnStart &s) {
+        const int lane = threadIdx.x & 31;
         request = s.request;
         q = attn_request(a, request);
-        const long long per_head = attn_head_tiles<ROWS, KEYS>(a, q);
+        const long long per_head = attn_head_tiles_warp<ROWS, KEYS>(a, q);
         const long long in = s.begin - s.request_begin;
         head = (int)(in / per_head);
         item_begin = s.request_begin + head * per_head;
-        for (tile = 0;; ++tile) {
-            attn_key_tiles<ROWS, KEYS>(a, q, tile, first, count);
-            if (s.begin < item_begin + count) break;
-            item_begin += count;
+        for (tile = 0; (long long)tile * ROWS < q.rows; tile += 32) {
+            int f = 0, n = 0;
+            if ((long long)(tile + lane) * ROWS < q.rows) attn_key_tiles<ROWS, KEYS>(a, q, tile + lane, f, n);
+            long long inc = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, s.begin < item_begin + inc);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                tile += l, item_begin += __shfl_sync(0xffffffffu, inc - n, l);
+                first = __shfl_sync(0xffffffffu, f, l), count = __shfl_sync(0xffffffffu, n, l);
+                break;
+            }
+            item_begin += __shfl_sync(0xffffffffu, inc, 31);
         }
         clip(s);
     }

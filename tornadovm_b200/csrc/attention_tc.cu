@@ -1,19 +1,21 @@
 // Attention of chunks of new tokens over a paged cache on the 5th-generation tensor cores.
 //
 // One persistent block per SM works on tiles of 256 query rows (two of 128, one per lane of tensor memory) against key
-// tiles of 128:
-//   * warp 8 fetches K and V tiles into a ring of shared-memory slots, one TMA box per page and 64 columns (lanes look
+// tiles of 64:
+//   * warp 8 fetches K and V tiles into two rings of shared-memory slots, one TMA box per page and 64 columns (lanes look
 //     the pages up side by side, a tile ahead); a page that no row sees, or that is none of the cache's, is fetched from
 //     behind the end of the tensor map and arrives as zeros;
-//   * warp 9 issues tcgen05.mma: S_t = Q_t K^T into tensor memory (fp32), and O_t += P_t V with P_t read from tensor
-//     memory, where it overlies S_t;
+//   * warps 9 and 10 issue the tcgen05.mma of one row tile each: S = Q K^T into tensor memory (fp32), and O += P V with P read from tensor memory, where
+//     it overlies S.  Each row tile has two score buffers: the product of key tile n + 2 follows that of P(n) V, so that
+//     the scores of tile n + 1 are there when the softmax is done with tile n and never waits in the steady state;
 //   * warps 0-3 and 4-7 hold the softmax of one 128-row tile each, a row per thread: S from tensor memory, the running
-//     maximum and sum in registers, P back as 16-bit values.  While one tile's probabilities are computed the tensor
-//     cores work on the other tile.  O stays in tensor memory; it is rescaled only when a row's maximum has grown by
-//     more than 2^8 since its reference was set (P then reaches 256 at most, well inside fp16, and the quotient O / l
-//     does not depend on the reference), which after the first tiles of a row hardly ever happens.
-// Bound: two products of 128 x 128 x head_dim and 128 x 128 powers of two per (row tile, key tile).  The key tiles of all
-// items are divided evenly over the blocks and split rows are joined afterwards (attention.cuh).
+//     maximum and sum in registers, P back as 16-bit values.  O stays in tensor memory; it is rescaled only when a row's
+//     maximum has grown by more than 2^8 since its reference was set (P then reaches 256 at most, well inside fp16, and
+//     the quotient O / l does not depend on the reference), which after the first tiles of a row hardly ever happens.
+// Bound: per row tile and key tile two products of 128 x 64 x head_dim, and 128 x 64 powers of two.  The key tiles of all
+// items are divided evenly over the blocks and split rows are joined afterwards (attention.cuh).  Code that runs once an
+// item stays in rolled loops: unrolled, its instructions arrived from L2 at 15 cycles each (fetching the query rows took
+// 15,000 cycles, more than the products of three key tiles).
 //
 // Every wait is bounded: on expiry the block records TB200_ERR_TIMEOUT, all roles leave their loops, copies in flight are
 // waited for (bounded again) and tensor memory is released.
@@ -25,25 +27,72 @@ TB200_TU_STATUS(attention_tc)
 
 namespace tb200 {
 
-constexpr int TC_ROWS = 256, TC_KEYS = 128, TC_THREADS = 384;  // three warpgroups; the last one's warps 8 and 9 work
-// Registers: 384 threads are launched with 168 each, which the softmax threads (128 scores in registers) outgrow, so the
-// warpgroups share them anew: 2 * 216 + 72 = 3 * 168.
-constexpr int TC_SOFTMAX_REGS = 216, TC_OTHER_REGS = 72;
+// Of every TC_POLY_OF pairs of probabilities, TC_POLY are computed on the FP32 pipe instead of the special-function unit.
+constexpr int TC_POLY = 1, TC_POLY_OF = 4;
+constexpr int TC_ROWS = 256, TC_KEYS = 64, TC_THREADS = 384;  // three warpgroups; the last one's warps 8 to 10 work
+// Registers: 384 threads are launched with 168 each, which the softmax threads (64 scores and 32 words of P in registers) outgrow, so the
+// warpgroups share them anew: 2 * 192 + 120 = 3 * 168.
+constexpr int TC_SOFTMAX_REGS = 192, TC_OTHER_REGS = 120;
 static_assert(2 * TC_SOFTMAX_REGS + TC_OTHER_REGS == 3 * 168, "the shares add up to what the block was launched with");
 
 template <int DPAD>
 struct TcShape {
-    static constexpr int PANELS = DPAD / 64;                // 64 columns = 128 bytes: the swizzled rows of a tile
-    static constexpr int PANEL_BYTES = TC_KEYS * 128;
-    static constexpr int TILE_BYTES = PANELS * PANEL_BYTES;  // K or V tile, and 128 query rows
-    static constexpr int SLOTS = DPAD == 128 ? 5 : 10;
-    static constexpr int SMEM = (2 + SLOTS) * TILE_BYTES + 1024;
+    static constexpr int PANELS = DPAD / 64;  // 64 columns = 128 bytes: the swizzled rows of a tile
+    static constexpr int KV_PANEL = TC_KEYS * 128, KV_BYTES = PANELS * KV_PANEL;   // K or V tile
+    static constexpr int Q_PANEL = 128 * 128, Q_BYTES = PANELS * Q_PANEL;          // 128 query rows
+    static constexpr int SLOTS = DPAD == 128 ? 5 : 10;                             // of K and of V
+    static constexpr int SMEM = 2 * Q_BYTES + 2 * SLOTS * KV_BYTES + 1024;
     static constexpr int GRID = 148;
     static constexpr size_t PART_FLOATS = (size_t)TC_ROWS * (DPAD + 2);
     static constexpr size_t WORKSPACE = GRID * sizeof(int4) + GRID * 2 * PART_FLOATS * 4;
-    // tensor memory: S_0, S_1 (128 columns each; P_t in the first 64 of S_t), O_0, O_1
+    // tensor memory: two score buffers of 64 columns for each row tile (P in the first 32 of a buffer), then O_0 and O_1
     static constexpr uint32_t O_COL = 256, TMEM_COLS = 512;
 };
+
+// ---- pairs of floats: the packed fp32 instructions do two at once ----
+__device__ __forceinline__ uint64_t tc_pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void tc_split(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t tc_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x on the FP32 pipe, for x <= 16; the special-function unit gives 16 powers a cycle and SM, which alone would take as
+// long as both products of a tile.  x = n + f with n = round(x) (by adding 1.5 * 2^23), |f| <= 1/2; 2^f is a polynomial
+// of degree 4 with p(0) = 1, fitted to the smallest largest relative error (2.9e-6, below the rounding of P by a factor
+// of 80 at least); n goes into the exponent.  x is held at -127, where the sum of exponents is that of zero: masked
+// scores give 0.
+__device__ __forceinline__ void tc_ex2_pair(uint64_t x2, float &p0, float &p1) {
+    float x, y;
+    tc_split(x2, x, y);
+    x2 = tc_pair(fmaxf(x, -127.0f), fmaxf(y, -127.0f));
+    const uint64_t n2 = tc_add2(x2, tc_pair(12582912.0f, 12582912.0f));
+    const uint64_t f2 = tc_fma2(tc_add2(n2, tc_pair(-12582912.0f, -12582912.0f)), tc_pair(-1.0f, -1.0f), x2);
+    uint64_t p2 = tc_fma2(f2, tc_pair(0.009582853f, 0.009582853f), tc_pair(0.055906426f, 0.055906426f));
+    p2 = tc_fma2(p2, f2, tc_pair(0.24024099f, 0.24024099f));
+    p2 = tc_fma2(p2, f2, tc_pair(0.69312418f, 0.69312418f));
+    p2 = tc_fma2(p2, f2, tc_pair(1.0f, 1.0f));
+    float n0, n1;
+    tc_split(n2, n0, n1);
+    tc_split(p2, p0, p1);
+    p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
+    p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
+}
+// the largest of three, NaN if one of them is
+__device__ __forceinline__ float tc_max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 __device__ __forceinline__ float tc_ex2(float x) {
     float r;
@@ -61,13 +110,14 @@ __device__ __forceinline__ uint32_t tc_finite_only(uint32_t w, __nv_bfloat16) {
 }
 
 struct TcShared {
-    uint64_t slot_full[10], slot_empty[10], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    uint64_t k_full[10], k_empty[10], v_full[10], v_empty[10];
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drained[2];  // [row tile][score buffer]
     AttnStart start;
-    long long scan[TC_THREADS / 32 + 1];
+    long long scan[32];
     uint32_t tmem_base;
     int abort_flag;
     int odd_values;        // some value of V at an edge was not finite: the rows that see it get it in the epilogue
-    uint32_t holes[8];     // per key tile (a ring): pages of the tile that are none of the cache's
+    uint32_t holes[16];    // per key tile (a ring): pages of the tile that are none of the cache's
 };
 
 // What the rows of an item see.
@@ -90,14 +140,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     extern __shared__ __align__(128) unsigned char tc_smem[];
     __shared__ __align__(16) TcShared sh;
     unsigned char *q_s = reinterpret_cast<unsigned char *>(((uintptr_t)tc_smem + 1023) & ~(uintptr_t)1023);  // swizzled tiles: 1024-byte bases
-    unsigned char *kv_s = q_s + 2 * S::TILE_BYTES;
+    unsigned char *k_s = q_s + 2 * S::Q_BYTES, *v_s = k_s + SLOTS * S::KV_BYTES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         sh.abort_flag = 0, sh.odd_values = 0;
-        for (int i = 0; i < SLOTS; ++i) mbar_init(&sh.slot_full[i], 1), mbar_init(&sh.slot_empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&sh.q_full[i], 128), mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_full[i], 4), mbar_init(&sh.o_full[i], 1);
-        mbar_init(&sh.drained, 1);
+        for (int i = 0; i < SLOTS; ++i) mbar_init(&sh.k_full[i], 1), mbar_init(&sh.k_empty[i], 2), mbar_init(&sh.v_full[i], 1), mbar_init(&sh.v_empty[i], 2);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.q_full[i], 128), mbar_init(&sh.pv_done[i], 1), mbar_init(&sh.o_full[i], 1), mbar_init(&sh.drained[i], 1);
+            for (int b = 0; b < 2; ++b) mbar_init(&sh.s_full[i][b], 1), mbar_init(&sh.p_full[i][b], 4);
+        }
         mbar_fence_init();
     }
     if (warp == 8 && lane == 0) tma_prefetch_map(&map_k), tma_prefetch_map(&map_v);
@@ -126,115 +178,139 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         // ---------------- producer ----------------
         const int box_keys = min(a.page_size, TC_KEYS), boxes = TC_KEYS / box_keys;
         const int behind = a.num_pages * a.kv_heads * a.page_size;  // first row behind the cache: zeros
-        uint32_t it = 0, tiles = 0;
+        uint32_t nk = 0, nv = 0;
+        // one tile: a box per page and panel, from the row that the box's lane has looked up
+        auto fetch = [&](const CUtensorMap *map, unsigned char *ring, uint64_t *full, uint64_t *empty, uint32_t &n, int row) {
+            const int s = n % SLOTS;
+            const uint32_t use = n / SLOTS;
+            if (use > 0 && !__all_sync(0xffffffffu, mbar_wait_abortable(&empty[s], (use - 1) & 1, abortp))) return false;
+            if (lane == 0) mbar_expect_tx(&full[s], S::KV_BYTES);
+            __syncwarp();
+            const int y = __shfl_sync(0xffffffffu, row, lane / PANELS);
+            if (lane < boxes * PANELS)
+                tma_load_2d(ring + s * S::KV_BYTES + (lane % PANELS) * S::KV_PANEL + (lane / PANELS) * box_keys * 128, map, (lane % PANELS) * 64, y, &full[s]);
+            ++n;
+            return true;
+        };
         while (more && ok) {
             const TcItem t(a, w);
             const int32_t *table = a.block_table + (long long)w.request * a.max_pages;
             // lane b: row of the cache at which box b of a tile begins, and whether its page is missing
-            auto look_up = [&](int tile, bool &hole) -> int {
-                const int key = tile * TC_KEYS + lane * box_keys;
+            auto look_up = [&](int n, bool &hole) -> int {
+                const int key = (t.tile0 + n) * TC_KEYS + lane * box_keys;
                 hole = false;
-                if (lane >= boxes || key > t.key_hi || key + box_keys <= t.key_lo) return behind;
+                if (n >= t.ntiles || lane >= boxes || key > t.key_hi || key + box_keys <= t.key_lo) return behind;
                 const int index = key >> a.page_shift, page = table[index];
                 hole = page < 0 || page >= a.num_pages;
                 return hole ? behind : (page * a.kv_heads + w.head) * a.page_size + (key - (index << a.page_shift));
             };
-            bool hole;
-            int row = look_up(t.tile0, hole);
-            for (int j = 0; j < t.ntiles && ok; ++j, ++tiles) {
-                bool next_hole = false;
-                const int next_row = j + 1 < t.ntiles ? look_up(t.tile0 + j + 1, next_hole) : behind;
-                const uint32_t holes = __ballot_sync(0xffffffffu, hole);
-                if (lane == 0) sh.holes[tiles & 7] = holes;
+            // order of use: K(0), K(1), V(0), K(2), V(1), ...
+            bool hole[3];
+            int row[3];
 #pragma unroll
-                for (int kv = 0; kv < 2; ++kv, ++it) {
-                    const int s = it % SLOTS;
-                    const uint32_t use = it / SLOTS;
-                    if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.slot_empty[s], (use - 1) & 1, abortp));
-                    if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(&sh.slot_full[s], S::TILE_BYTES);
-                    __syncwarp();
-                    for (int i = lane; i < ((boxes * PANELS + 31) & ~31); i += 32) {
-                        const int b = i / PANELS, panel = i % PANELS;
-                        const int y = __shfl_sync(0xffffffffu, row, b & 31);
-                        if (b < boxes)
-                            tma_load_2d(kv_s + s * S::TILE_BYTES + panel * S::PANEL_BYTES + b * box_keys * 128, kv == 0 ? &map_k : &map_v, panel * 64, y,
-                                        &sh.slot_full[s]);
-                    }
-                }
-                row = next_row, hole = next_hole;
+            for (int i = 0; i < 2; ++i) row[i] = look_up(i, hole[i]);
+            auto fetch_k = [&](int r, bool h) {
+                const uint32_t holes = __ballot_sync(0xffffffffu, h);
+                if (lane == 0) sh.holes[nk & 15] = holes;
+                return fetch(&map_k, k_s, sh.k_full, sh.k_empty, nk, r);
+            };
+            ok = fetch_k(row[0], hole[0]) && (t.ntiles < 2 || fetch_k(row[1], hole[1]));
+#pragma unroll 1
+            for (int n = 0; n < t.ntiles && ok; ++n) {
+                row[2] = look_up(n + 2, hole[2]);
+                ok = fetch(&map_v, v_s, sh.v_full, sh.v_empty, nv, row[0]);
+                if (ok && n + 2 < t.ntiles) ok = fetch_k(row[2], hole[2]);
+                row[0] = row[1], row[1] = row[2];
             }
             more = w.next(a, sh.start);
         }
         // copies in flight when a wait has expired (in the normal course all have been waited for by their readers)
-        if (!ok && lane == 0)
-            for (uint32_t k = it > SLOTS ? it - SLOTS : 0; k < it; ++k)
-                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sh.slot_full[k % SLOTS], (k / SLOTS) & 1); ++i) {
+        if (!ok && lane == 0) {
+            for (uint32_t k = nk > SLOTS ? nk - SLOTS : 0; k < nk; ++k)
+                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sh.k_full[k % SLOTS], (k / SLOTS) & 1); ++i) {
                 }
-    } else if (warp == 9) {
-        // ---------------- products ----------------
-        if (lane == 0) {
-            uint32_t it = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
-            const uint32_t q_addr = smem_u32(q_s), kv_addr = smem_u32(kv_s);
-            // S_t = Q_t K^T: both operands K-major, rows of 128 bytes, 16 columns = 32 bytes per instruction
-            auto qk = [&](int t, uint32_t slot) {
+            for (uint32_t k = nv > SLOTS ? nv - SLOTS : 0; k < nv; ++k)
+                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sh.v_full[k % SLOTS], (k / SLOTS) & 1); ++i) {
+                }
+        }
+    } else if (warp <= 10) {
+        // ---------------- products, a warp per row tile ----------------
+        // (Each wait of a warp costs it some 250 cycles even where nothing is left to wait for, and products are issued at
+        // the rate at which they run: with one warp for both tiles the tensor cores idled half of the time.)
+        // ----------------
+        // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.
+        const int t = warp - 9;
+        const bool leader = lane == 0;
+        uint32_t nk = 0, nv = 0, q_use = 0, g_s = 0, g_p = 0;  // key tiles of the block so far; items and score tiles (begun, used) of the row tile
+        const uint64_t q_desc = make_smem_desc(smem_u32(q_s) + t * S::Q_BYTES, 16, 1024), k_desc = make_smem_desc(smem_u32(k_s), 16, 1024);
+        const uint64_t v_desc = make_smem_desc(smem_u32(v_s), S::KV_PANEL, 1024);
+        // S = Q K^T: both operands K-major, rows of 128 bytes, 16 columns = 32 bytes per instruction
+        auto qk = [&](uint32_t slot) {
+            const uint64_t k = k_desc + (uint64_t)(slot * (S::KV_BYTES >> 4));
+            const uint32_t b = g_s++ & 1, d = tmem + t * 128 + b * 64;
+            if (leader) {
 #pragma unroll
-                for (int k = 0; k < DPAD / 16; ++k) {
-                    const uint32_t at = (k / 4) * S::PANEL_BYTES + (k % 4) * 32;
-                    tc_mma_f16(tmem + t * 128, make_smem_desc(q_addr + t * S::TILE_BYTES + at, 16, 1024), make_smem_desc(kv_addr + slot * S::TILE_BYTES + at, 16, 1024),
-                               idesc_qk, k > 0);
-                }
-                tc_commit(&sh.s_full[t]);
-            };
-            // O_t (+)= P_t V: P in tensor memory (16 keys = 8 columns), V with its columns contiguous, 16 keys = 2048 bytes
-            auto pv = [&](int t, uint32_t slot, bool add) {
-                const uint64_t v = make_smem_desc(kv_addr + slot * S::TILE_BYTES, S::PANEL_BYTES, 1024);
+                for (int i = 0; i < DPAD / 16; ++i)
+                    tc_mma_f16(d, q_desc + (uint64_t)(((i / 4) * S::Q_PANEL + (i % 4) * 32) >> 4), k + (uint64_t)(((i / 4) * S::KV_PANEL + (i % 4) * 32) >> 4), idesc_qk, i > 0);
+                tc_commit(&sh.s_full[t][b]);
+                tc_commit(&sh.k_empty[slot]);
+            }
+        };
+        // O (+)= P V: P in tensor memory (16 keys = 8 columns), V with its columns contiguous, 16 keys = 2048 bytes
+        auto pv = [&](uint32_t slot, bool add) {
+            const uint64_t v = v_desc + (uint64_t)(slot * (S::KV_BYTES >> 4));
+            const uint32_t b = g_p & 1, p = tmem + t * 128 + b * 64, d = tmem + S::O_COL + t * 128;
+            if (!__all_sync(0xffffffffu, mbar_wait_abortable(&sh.p_full[t][b], (g_p >> 1) & 1, abortp))) return false;
+            ++g_p;
+            tc_fence_after();
+            if (leader) {
 #pragma unroll
-                for (int k = 0; k < TC_KEYS / 16; ++k) tc_mma_f16_ta(tmem + S::O_COL + t * 128, tmem + t * 128 + k * 8, v + (uint64_t)(k * 128), idesc_pv, add || k > 0);
-            };
-            auto wait_slot = [&]() { return mbar_wait_abortable(&sh.slot_full[it % SLOTS], (it / SLOTS) & 1, abortp); };
-            auto wait_p = [&](int t) {
-                const bool r = mbar_wait_abortable(&sh.p_full[t], p_use[t]++ & 1, abortp);
-                tc_fence_after();
-                return r;
-            };
-            while (more && ok) {
-                const TcItem t(a, w);
-                const bool two = t.rows > 128;
-                ok = mbar_wait_abortable(&sh.q_full[0], q_use[0]++ & 1, abortp) && (!two || mbar_wait_abortable(&sh.q_full[1], q_use[1]++ & 1, abortp));
-                uint32_t v_slot = 0;
-                for (int j = 0; j < t.ntiles && ok; ++j) {
-                    const uint32_t k_slot = it % SLOTS;
-                    if (!(ok = wait_slot())) break;
-                    tc_fence_after();
-                    ++it;
-                    qk(0, k_slot);
-                    if (two) {
-                        if (j > 0) {
-                            if (!(ok = wait_p(1))) break;
-                            pv(1, v_slot, j > 1);
-                            tc_commit(&sh.slot_empty[v_slot]);
-                        }
-                        qk(1, k_slot);
-                    }
-                    tc_commit(&sh.slot_empty[k_slot]);
-                    v_slot = it % SLOTS;
-                    if (!(ok = wait_slot())) break;
-                    ++it;
-                    if (!(ok = wait_p(0))) break;
-                    pv(0, v_slot, j > 0);
-                    if (!two) tc_commit(&sh.slot_empty[v_slot]);
-                }
-                if (ok) tc_commit(&sh.o_full[0]);
-                if (ok && two && (ok = wait_p(1))) {
-                    pv(1, v_slot, t.ntiles > 1);
-                    tc_commit(&sh.slot_empty[v_slot]);
-                    tc_commit(&sh.o_full[1]);
+                for (int i = 0; i < TC_KEYS / 16; ++i) tc_mma_f16_ta(d, p + i * 8, v + (uint64_t)(i * 128), idesc_pv, add || i > 0);
+                tc_commit(&sh.pv_done[t]);
+                tc_commit(&sh.v_empty[slot]);
+            }
+            return true;
+        };
+        auto wait_full = [&](uint64_t *full, uint32_t n) {
+            const bool r = __all_sync(0xffffffffu, mbar_wait_abortable(&full[n % SLOTS], (n / SLOTS) & 1, abortp));
+            tc_fence_after();
+            return r;
+        };
+        while (more && ok) {
+            const TcItem im(a, w);
+            if (t == 1 && im.rows <= 128) {  // nothing to multiply: this warp's share of the slots is released in turn
+#pragma unroll 1
+                for (int n = 0; n < im.ntiles && ok; ++n) {
+                    ok = wait_full(sh.k_full, nk);
+                    if (ok && leader) mbar_arrive(&sh.k_empty[nk % SLOTS]);
+                    ++nk;
+                    ok = ok && wait_full(sh.v_full, nv);
+                    if (ok && leader) mbar_arrive(&sh.v_empty[nv % SLOTS]);
+                    ++nv;
                 }
                 more = w.next(a, sh.start);
+                continue;
             }
-            tc_commit(&sh.drained);  // nothing of this block's products is under way when tensor memory is released
-            for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sh.drained, 0); ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.q_full[t], q_use++ & 1, abortp));
+#pragma unroll 1
+            for (int n = 0; n < min(2, im.ntiles) && ok; ++n) {
+                if (!(ok = wait_full(sh.k_full, nk))) break;
+                qk(nk++ % SLOTS);
+            }
+#pragma unroll 1
+            for (int n = 0; n < im.ntiles && ok; ++n) {
+                const bool next = n + 2 < im.ntiles;
+                if (!(ok = wait_full(sh.v_full, nv))) break;
+                if (next && !(ok = wait_full(sh.k_full, nk))) break;
+                if (!(ok = pv(nv++ % SLOTS, n > 0))) break;
+                if (next) qk(nk++ % SLOTS);
+                else if (n + 1 == im.ntiles && leader) tc_commit(&sh.o_full[t]);
+            }
+            more = w.next(a, sh.start);
+        }
+        if (leader) {
+            tc_commit(&sh.drained[t]);  // nothing of this block's products is under way when tensor memory is released
+            for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sh.drained[t], 0); ++i) {
             }
         }
         __syncwarp();
@@ -244,73 +320,114 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         // ---------------- softmax ----------------
         const int t = warp >> 2, row_in = threadIdx.x & 127, D = a.head_dim, chunks = D / 8;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + S::O_COL + t * 128;
-        const bool q_vec = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 8 == 0;
-        unsigned char *my_q = q_s + t * S::TILE_BYTES;
-        uint32_t it = 0, tiles = 0, s_use = 0, o_use = 0;
-        while (more && ok) {
-            const TcItem im(a, w);
-            if (t == 1 && im.rows <= 128) {
-                it += 2 * im.ntiles, tiles += im.ntiles;
+        uint32_t nkv = 0, g = 0, o_use = 0;  // key tiles of the block so far, score tiles of this row tile, items of this row tile
+        // The next item that has rows for this tile: its query rows to shared memory by asynchronous copies (DPAD / 8
+        // threads share a row, so that the reads are whole lines).
+        auto take_item = [&]() {
+            while (more && t == 1 && w.q.rows - w.tile * TC_ROWS <= 128) {
+                nkv += w.to - w.from;
                 more = w.next(a, sh.start);
-                continue;
             }
-            // query rows: 8 threads of a warp share a row's 16-byte pieces, so that the reads are whole lines
-            for (int e = row_in; e < 128 * (DPAD / 8); e += 128) {
-                const int r = e / (DPAD / 8), c = e % (DPAD / 8), row = t * 128 + r, at = im.row0 + row;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < im.rows && c < chunks) {
-                    const int token = at / a.group, head = w.head * a.group + (at - token * a.group);
-                    const T *src = static_cast<const T *>(a.q) + (w.q.first + token) * a.q_stride + (long long)head * D + c * 8;
-                    if (q_vec) {
-                        v = *reinterpret_cast<const uint4 *>(src);
-                    } else {
-                        const uint16_t *h = reinterpret_cast<const uint16_t *>(src);
-                        v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
-                    }
+            if (!more) return;
+            constexpr int CPR = DPAD / 8, STEP = 128 / CPR;
+            const int c = row_in % CPR, r0 = row_in / CPR, row0 = w.tile * TC_ROWS + t * 128;
+            const bool q_vec = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 8 == 0;
+            const T *q = static_cast<const T *>(a.q) + w.q.first * a.q_stride + (long long)w.head * a.group * D + c * 8;
+            unsigned char *dst = q_s + t * S::Q_BYTES + (c >> 3) * S::Q_PANEL;
+            int token = (row0 + r0) / a.group, in = row0 + r0 - token * a.group;  // head of the group
+            const int token_step = STEP / a.group, in_step = STEP - token_step * a.group;
+#pragma unroll 1
+            for (int r = r0; r < 128; r += STEP) {
+                const bool there = row0 + r < w.q.rows && c < chunks;
+                const T *src = there ? q + token * a.q_stride + (long long)in * D : static_cast<const T *>(a.q);
+                token += token_step, in += in_step;
+                if (in >= a.group) in -= a.group, ++token;
+                unsigned char *at = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                if (q_vec) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at)), "l"(src), "r"(there ? 16 : 0) : "memory");
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t *>(at)[i] = there ? reinterpret_cast<const uint16_t *>(src)[i] : (uint16_t)0;
                 }
-                *reinterpret_cast<uint4 *>(my_q + (c >> 3) * S::PANEL_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_shared();
             mbar_arrive(&sh.q_full[t]);
-
+        };
+        take_item();
+        while (more && ok) {
+            const TcItem im(a, w);
             const int my_row = t * 128 + row_in;
             const bool have = my_row < im.rows, warp_has = t * 128 + (warp & 3) * 32 < im.rows;
             const int pos = have ? im.base + (im.row0 + my_row) / a.group : -1;
             const int see_hi = min(pos, w.q.visible - 1), see_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+            const uint64_t scale2 = tc_pair(a.scale_log2, a.scale_log2);
             float m = -INFINITY, l = 0.0f;
-            for (int j = 0; j < im.ntiles; ++j, ++tiles, it += 2) {
-                ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.s_full[t], s_use++ & 1, abortp));
+#pragma unroll 1
+            for (int n = 0; n < im.ntiles; ++n, ++nkv, ++g) {
+                const uint32_t b = g & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.s_full[t][b], (g >> 1) & 1, abortp));
                 if (!ok) break;
                 tc_fence_after();
-                const int key0 = (im.tile0 + j) * TC_KEYS;
-                const uint32_t holes = sh.holes[tiles & 7];
+                const int key0 = (im.tile0 + n) * TC_KEYS;
+                const uint32_t holes = sh.holes[nkv & 15];
                 const bool edge = key0 + TC_KEYS - 1 > min(im.pos_first, im.key_hi) || (a.window > 0 && key0 <= im.pos_last - a.window);
+                uint32_t s[64];
+                float top = -INFINITY;
                 if (warp_has) {
-                    uint32_t s[128];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tc_ld_32cols(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+                    tc_ld_32cols(s_addr + b * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                    tc_ld_32cols(s_addr + b * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
                     tc_wait_ld();
                     if (edge) {
                         const int lo = see_lo - key0, hi = see_hi - key0;
 #pragma unroll
-                        for (int i = 0; i < 128; ++i)
+                        for (int i = 0; i < 64; ++i)
                             if (i > hi || i < lo) s[i] = 0xFF800000u;
                     }
                     if (holes) {
-                        const int shift = min(a.page_shift, 7);
+                        const int shift = min(a.page_shift, 6);
 #pragma unroll
-                        for (int i = 0; i < 128; ++i)
+                        for (int i = 0; i < 64; ++i)
                             if ((holes >> (i >> shift)) & 1) s[i] = 0xFF800000u;
                     }
                     float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) x[i & 3] = fmaxf(x[i & 3], __uint_as_float(s[i]));
-                    const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale_log2;
-                    if (j == 0) {
+                    for (int i = 0; i < 64; i += 2) x[(i >> 1) & 3] = tc_max3(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                    top = tc_max3(tc_max3(x[0], x[1], x[2]), x[3], x[3]) * a.scale_log2;
+                }
+                if (edge) {
+                    // A place that no row sees may hold anything, and one that some rows see and others do not may hold
+                    // an infinity or a NaN: 0 * V would carry it to rows that do not see it.  The former become zeros
+                    // here; of the latter the values that are not finite do, and the epilogue gives them to their rows.
+                    // (Both tiles' warps do so, two threads a key; they write the same.)
+                    ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.v_full[nkv % SLOTS], (nkv / SLOTS) & 1, abortp));
+                    if (!ok) break;
+                    const int in = row_in >> 1, key = key0 + in;
+                    unsigned char *v_row = v_s + (nkv % SLOTS) * S::KV_BYTES + in * 128;
+                    const bool unseen = key > im.key_hi || key < im.key_lo;
+                    if (unseen || key > im.pos_first || (a.window > 0 && key <= im.pos_last - a.window)) {
+#pragma unroll 1
+                        for (int c = row_in & 1; c < DPAD / 8; c += 2) {
+                            uint4 *at = reinterpret_cast<uint4 *>(v_row + (c >> 3) * S::KV_PANEL + (((c & 7) ^ (in & 7)) << 4));
+                            const uint4 v = *at;
+                            const bool odd = tc_not_finite(v.x, T()) || tc_not_finite(v.y, T()) || tc_not_finite(v.z, T()) || tc_not_finite(v.w, T());
+                            if (odd && !unseen) sh.odd_values = 1;
+                            if (unseen) *at = make_uint4(0, 0, 0, 0);
+                            else if (odd) *at = make_uint4(tc_finite_only(v.x, T()), tc_finite_only(v.y, T()), tc_finite_only(v.z, T()), tc_finite_only(v.w, T()));
+                        }
+                    }
+                    fence_async_shared();
+                }
+                if (warp_has) {
+                    if (n == 0) {
                         m = top;
                     } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                        // the product before this one may still be adding to O
+                        ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.pv_done[t], (g - 1) & 1, abortp));
+                        if (!ok) break;
+                        tc_fence_after();
                         const float next = fmaxf(m, top), f = next == m ? 1.0f : tc_ex2(m - next);
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < DPAD / 32; ++c) {
                             uint32_t o[32];
                             tc_ld_32cols(o_addr + c * 32, o);
@@ -321,62 +438,50 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         }
                         l *= f, m = next;
                     }
-                    const float shift = m == -INFINITY ? 0.0f : m;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const float shift = m == -INFINITY ? 0.0f : -m;
+                    const uint64_t shift2 = tc_pair(shift, shift);
+                    uint64_t sum[2] = {0, 0};
+                    uint32_t p[32];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t p[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float p0 = tc_ex2(fmaf(__uint_as_float(s[64 * c + 2 * i]), a.scale_log2, -shift));
-                            const float p1 = tc_ex2(fmaf(__uint_as_float(s[64 * c + 2 * i + 1]), a.scale_log2, -shift));
-                            sum[i & 3] += p0 + p1;
-                            p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
+                    for (int i = 0; i < 32; ++i) {
+                        const uint64_t x2 = tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift2);
+                        float p0, p1;
+                        if (i % TC_POLY_OF < TC_POLY) {
+                            tc_ex2_pair(x2, p0, p1);
+                        } else {
+                            tc_split(x2, p0, p1);
+                            p0 = tc_ex2(p0), p1 = tc_ex2(p1);
                         }
-                        tc_st_32cols(s_addr + c * 32, p);
+                        sum[i & 1] = tc_add2(sum[i & 1], tc_pair(p0, p1));
+                        p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tc_st_32cols(s_addr + b * 64, p);
+                    float s0, s1;
+                    tc_split(tc_add2(sum[0], sum[1]), s0, s1);
+                    l += s0 + s1;
+                    if (!(top < INFINITY)) l = __int_as_float(0x7FC00000);  // a score of +infinity or NaN: the row is NaN
                     tc_wait_st();
-                }
-                if (edge) {
-                    // A place that no row sees may hold anything, and one that some rows see and others do not may hold
-                    // an infinity or a NaN: 0 * V would carry it to rows that do not see it.  The former become zeros
-                    // here; of the latter the values that are not finite do, and the epilogue gives them to their rows.
-                    ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.slot_full[(it + 1) % SLOTS], ((it + 1) / SLOTS) & 1, abortp));
-                    if (!ok) break;
-                    const int key = key0 + row_in;
-                    unsigned char *v_row = kv_s + ((it + 1) % SLOTS) * S::TILE_BYTES + row_in * 128;
-                    if (key > im.key_hi || key < im.key_lo) {
-#pragma unroll
-                        for (int c = 0; c < DPAD / 8; ++c) *reinterpret_cast<uint4 *>(v_row + (c >> 3) * S::PANEL_BYTES + (((c & 7) ^ (row_in & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-                    } else if (key > im.pos_first || (a.window > 0 && key <= im.pos_last - a.window)) {
-#pragma unroll
-                        for (int c = 0; c < DPAD / 8; ++c) {
-                            uint4 *at = reinterpret_cast<uint4 *>(v_row + (c >> 3) * S::PANEL_BYTES + (((c & 7) ^ (row_in & 7)) << 4));
-                            const uint4 v = *at;
-                            if (tc_not_finite(v.x, T()) || tc_not_finite(v.y, T()) || tc_not_finite(v.z, T()) || tc_not_finite(v.w, T())) {
-                                sh.odd_values = 1;
-                                *at = make_uint4(tc_finite_only(v.x, T()), tc_finite_only(v.y, T()), tc_finite_only(v.z, T()), tc_finite_only(v.w, T()));
-                            }
-                        }
-                    }
-                    fence_async_shared();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[t]);
+                if (lane == 0) mbar_arrive(&sh.p_full[t][b]);
             }
             if (!ok) break;
+            // All scores of the item have been read, so its query rows are done with: the next item's are fetched while
+            // the last products run.
+            const AttnWalk<TC_ROWS, TC_KEYS> done = w;
+            more = w.next(a, sh.start);
+            const bool last = !more;
+            take_item();
             ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.o_full[t], o_use++ & 1, abortp));
             if (!ok) break;
             tc_fence_after();
-            const bool whole = w.whole(), odd = *reinterpret_cast<volatile int *>(&sh.odd_values) != 0;
+            const bool whole = done.whole(), odd = *reinterpret_cast<volatile int *>(&sh.odd_values) != 0;
             if (warp_has) {
                 const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-                const int at = im.row0 + my_row, token = at / a.group, head = w.head * a.group + (at - token * a.group);
-                T *dst = static_cast<T *>(a.out) + (w.q.first + token) * a.out_stride + (long long)head * D;
-                const bool vec8 = ((uintptr_t)dst & 7) == 0;
-                float *part = a.parts + ((long long)blockIdx.x * 2 + (w.from == 0)) * S::PART_FLOATS + my_row;
+                const int at = im.row0 + my_row, token = at / a.group, head = done.head * a.group + (at - token * a.group);
+                T *dst = static_cast<T *>(a.out) + (done.q.first + token) * a.out_stride + (long long)head * D;
+                float *part = a.parts + ((long long)blockIdx.x * 2 + (done.from == 0)) * S::PART_FLOATS + my_row;
 #pragma unroll 1
                 for (int c = 0; c < DPAD / 32; ++c) {
                     uint32_t o[32];
@@ -387,9 +492,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         const int lo = max(max(see_lo, im.key_lo), im.tile0 * TC_KEYS), hi = min(see_hi, (im.tile0 + im.ntiles) * TC_KEYS - 1);
                         for (int key = lo; key <= hi; ++key) {
                             if (key <= im.pos_first && !(a.window > 0 && key <= im.pos_last - a.window)) continue;
-                            const int index = key >> a.page_shift, page = a.block_table[(long long)w.request * a.max_pages + index];
+                            const int index = key >> a.page_shift, page = a.block_table[(long long)done.request * a.max_pages + index];
                             if (page < 0 || page >= a.num_pages) continue;
-                            const T *v = static_cast<const T *>(a.v_cache) + (((long long)page * a.kv_heads + w.head) * a.page_size + (key - (index << a.page_shift))) * D;
+                            const T *v = static_cast<const T *>(a.v_cache) + (((long long)page * a.kv_heads + done.head) * a.page_size + (key - (index << a.page_shift))) * D;
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
                                 const float f = c * 32 + i < D ? to_f32(v[c * 32 + i]) : 0.0f;
@@ -401,25 +506,39 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                         for (int i = 0; i < 32; ++i) part[(c * 32 + i) * TC_ROWS] = __uint_as_float(o[i]);
                     } else if (have) {
+                        uint32_t h[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            if (c * 32 + i >= D) break;
-                            const float f[4] = {__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv, __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv};
-                            if (vec8) {
-                                *reinterpret_cast<uint2 *>(dst + c * 32 + i) = make_uint2(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()));
+                        for (int i = 0; i < 16; ++i) h[i] = pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv, T());
+                        T *d = dst + c * 32;
+                        const uintptr_t phase = (uintptr_t)d;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {  // pieces of 8 columns
+                            if (c * 32 + i * 8 >= D) break;
+                            if ((phase & 15) == 0) {
+                                *reinterpret_cast<uint4 *>(d + i * 8) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
                             } else {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) from_f32(dst[c * 32 + i + e], f[e]);
+                                for (int k = 0; k < 4; ++k) {
+                                    if ((phase & 3) == 0) {
+                                        *reinterpret_cast<uint32_t *>(d + i * 8 + 2 * k) = h[4 * i + k];
+                                    } else {
+                                        reinterpret_cast<uint16_t *>(d)[i * 8 + 2 * k] = (uint16_t)h[4 * i + k];
+                                        reinterpret_cast<uint16_t *>(d)[i * 8 + 2 * k + 1] = (uint16_t)(h[4 * i + k] >> 16);
+                                    }
+                                }
                             }
                         }
                     }
                 }
                 if (!whole) part[DPAD * TC_ROWS] = m, part[(DPAD + 1) * TC_ROWS] = l;
             }
-            if (!whole && w.from == 0 && threadIdx.x == 0)
-                a.joins[blockIdx.x] = make_int4(w.request, w.head, w.tile, attn_block_of(sh.start.total, sh.start.blocks, w.item_begin + w.count - 1));
-            more = w.next(a, sh.start);
-            if (!more && (whole || w.from != 0) && threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+            if (threadIdx.x == 0) {
+                if (!whole && done.from == 0)
+                    a.joins[blockIdx.x] = make_int4(done.request, done.head, done.tile, attn_block_of(sh.start.total, sh.start.blocks, done.item_begin + done.count - 1));
+                else if (last)
+                    a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+            }
+            tc_fence_before();  // this item's O has been read before the next one's products are let on it
         }
         if (!ok && threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
         tc_fence_before();
