@@ -18,6 +18,7 @@ TB200_TU_STATUS(attention)
 namespace tb200 {
 
 constexpr int AT_THREADS = 128, AT_KEYS = 64;
+constexpr int AT_ITEM = 1;       // what an item costs besides its key tiles, in such tiles
 constexpr int AT_TC_ROWS = 64;   // requests of more rows go to the tensor-memory kernel
 constexpr int AT_MAX_SMS = 148;  // the workspace is sized without asking the device
 
@@ -90,17 +91,16 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
     const int warp_key = SPLIT_KEYS ? warp * 16 : 0, warp_row = SPLIT_KEYS ? 0 : warp * 16;
     const bool copy16 = ((uintptr_t)a.k_cache & 15) == 0 && ((uintptr_t)a.v_cache & 15) == 0;
 
-    attn_find_start<AT_THREADS, ROWS, AT_KEYS>(a, &start, scan);
+    attn_find_start<AT_THREADS, ROWS, AT_KEYS, AT_ITEM>(a, &start, scan);
     if (start.begin >= start.end) {
         if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
         pdl_launch_dependents();
         return;
     }
-    AttnWalk<ROWS, AT_KEYS> w;
-    w.seek(a, start);
+    AttnWalk<ROWS, AT_KEYS, AT_ITEM> w;
+    bool more = w.seek(a, start);
     int4 join = make_int4(-1, 0, 0, 0);
 
-    bool more = true;
     while (more) {
         const AttnRequest rq = w.q;
         const int row0 = w.tile * ROWS, rows = min(ROWS, rq.rows - row0), base = rq.kv_len - rq.new_tokens;
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
 
         const bool whole = w.whole();
         if (!whole && w.from == 0 && tid == 0)
-            join = make_int4(w.request, w.head, w.tile, attn_block_of(start.total, start.blocks, w.item_begin + w.count - 1));
+            join = make_int4(w.request, w.head, w.tile, attn_block_of(start.total, start.blocks, w.item_begin + AT_ITEM + w.count - 1));
         float *part = a.parts + ((long long)blockIdx.x * 2 + (w.from == 0)) * S::PART_FLOATS;
         // one row's columns d, d + 1 of the result or of the part
         const bool out2 = ((uintptr_t)a.out & 3) == 0 && a.out_stride % 2 == 0;

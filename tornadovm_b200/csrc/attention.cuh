@@ -8,6 +8,9 @@
 // lengths are.  Lengths live on the device, so each block repeats the prefix sum over the requests by itself (reads
 // that L2 serves), and no block waits for another.
 //
+// An item counts as its key tiles and ITEM tiles more that stand for what it costs besides; these come first and have no
+// keys, so a block that ends inside them leaves the item to the next block altogether.
+//
 // A block that holds a whole item normalises and stores it.  Otherwise it leaves the running maximum, sum and
 // unnormalised output of its part in the workspace, in one of two places that belong to the block: 0 for an item that
 // an earlier block began, 1 for an item that it begins itself.  A second kernel joins the parts in the order of blocks.
@@ -59,23 +62,23 @@ __device__ __forceinline__ void attn_key_tiles(const AttnArgs &a, const AttnRequ
 }
 
 // Key tiles of all row tiles of a request for one head: by one thread, and by a warp.
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int ITEM>
 __device__ __forceinline__ long long attn_head_tiles(const AttnArgs &a, const AttnRequest &q) {
     long long n = 0;
     for (int t = 0; (long long)t * ROWS < q.rows; ++t) {
         int first, count;
         attn_key_tiles<ROWS, KEYS>(a, q, t, first, count);
-        n += count;
+        n += ITEM + count;
     }
     return n;
 }
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int ITEM>
 __device__ __forceinline__ long long attn_head_tiles_warp(const AttnArgs &a, const AttnRequest &q) {
     long long n = 0;
     for (int t = threadIdx.x & 31; (long long)t * ROWS < q.rows; t += 32) {
         int first, count;
         attn_key_tiles<ROWS, KEYS>(a, q, t, first, count);
-        n += count;
+        n += ITEM + count;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
@@ -84,9 +87,16 @@ __device__ __forceinline__ long long attn_head_tiles_warp(const AttnArgs &a, con
 
 // First tile of block `b` of `blocks` over `total` tiles, and the block that has tile `u`.  blocks <= total: every block
 // between two that share an item has a part of it.
-__device__ __forceinline__ long long attn_block_begin(long long total, int b, int blocks) { return total / blocks * b + total % blocks * b / blocks; }
+// (64-bit divisions are subroutines of some hundred instructions: calls of less than 2^32 tiles, which all are, avoid them.)
+__device__ __forceinline__ long long attn_div(long long n, long long d) {
+    return ((n | d) >> 32) == 0 ? (long long)((unsigned)n / (unsigned)d) : n / d;
+}
+__device__ __forceinline__ long long attn_block_begin(long long total, int b, int blocks) {
+    const long long each = attn_div(total, blocks);
+    return each * b + (unsigned)(total - each * blocks) * (unsigned)b / (unsigned)blocks;
+}
 __device__ __forceinline__ int attn_block_of(long long total, int blocks, long long u) {
-    int b = (int)min((long long)blocks - 1, u * blocks / total);  // exact up to rounding: step to the block that has it
+    int b = (int)min((long long)blocks - 1, attn_div(u * blocks, total));  // exact up to rounding: step to the block that has it
     while (b > 0 && attn_block_begin(total, b, blocks) > u) --b;
     while (b + 1 < blocks && attn_block_begin(total, b + 1, blocks) <= u) ++b;
     return b;
@@ -101,7 +111,7 @@ struct AttnStart {
 
 // Run by all threads of the block; `scan`: 32 words of shared memory.  Few requests are counted by a warp each (a long
 // prompt has hundreds of row tiles), many by a thread each.
-template <int THREADS, int ROWS, int KEYS>
+template <int THREADS, int ROWS, int KEYS, int ITEM>
 __device__ __forceinline__ void attn_find_start(const AttnArgs &a, AttnStart *out, long long *scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool few = a.requests <= 32;
@@ -109,7 +119,7 @@ __device__ __forceinline__ void attn_find_start(const AttnArgs &a, AttnStart *ou
     int r0 = 0, r1 = 0;
     if (few) {
         for (int r = warp; r < a.requests; r += THREADS / 32) {
-            const long long n = attn_head_tiles_warp<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
+            const long long n = attn_head_tiles_warp<ROWS, KEYS, ITEM>(a, attn_request(a, r)) * a.kv_heads;
             if (lane == 0) scan[r] = n;
         }
         __syncthreads();
@@ -117,7 +127,7 @@ __device__ __forceinline__ void attn_find_start(const AttnArgs &a, AttnStart *ou
     } else {
         const int per = (a.requests + THREADS - 1) / THREADS;
         r0 = min(a.requests, (int)threadIdx.x * per), r1 = min(a.requests, r0 + per);
-        for (int r = r0; r < r1; ++r) mine += attn_head_tiles<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
+        for (int r = r0; r < r1; ++r) mine += attn_head_tiles<ROWS, KEYS, ITEM>(a, attn_request(a, r)) * a.kv_heads;
     }
     long long inc = mine;
 #pragma unroll
@@ -144,7 +154,7 @@ __device__ __forceinline__ void attn_find_start(const AttnArgs &a, AttnStart *ou
         long long at = before;
         int r = few ? lane : r0;
         for (; !few && r < r1; ++r) {
-            const long long n = attn_head_tiles<ROWS, KEYS>(a, attn_request(a, r)) * a.kv_heads;
+            const long long n = attn_head_tiles<ROWS, KEYS, ITEM>(a, attn_request(a, r)) * a.kv_heads;
             if (begin < at + n) break;
             at += n;
         }
@@ -154,7 +164,7 @@ __device__ __forceinline__ void attn_find_start(const AttnArgs &a, AttnStart *ou
 }
 
 // The block's walk over its items.
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int ITEM>
 struct AttnWalk {
     AttnRequest q;
     int request, head, tile;    // the item
@@ -162,19 +172,21 @@ struct AttnWalk {
     int from, to;               // this block's of them: [from, to) of [0, count)
     long long item_begin;       // the item's first tile in the call
 
-    // The item that holds the block's first tile; run by whole warps, whose lanes look at 32 row tiles at a time.
-    __device__ __forceinline__ void seek(const AttnArgs &a, const AttnStart &s) {
+    // The first item of which the block has key tiles, false if there is none; run by whole warps, whose lanes look at 32
+    // row tiles at a time.
+    __device__ __forceinline__ bool seek(const AttnArgs &a, const AttnStart &s) {
         const int lane = threadIdx.x & 31;
         request = s.request;
         q = attn_request(a, request);
-        const long long per_head = attn_head_tiles_warp<ROWS, KEYS>(a, q);
+        const long long per_head = attn_head_tiles_warp<ROWS, KEYS, ITEM>(a, q);
         const long long in = s.begin - s.request_begin;
-        head = (int)(in / per_head);
+        head = (int)attn_div(in, per_head);
         item_begin = s.request_begin + head * per_head;
         for (tile = 0; (long long)tile * ROWS < q.rows; tile += 32) {
             int f = 0, n = 0;
             if ((long long)(tile + lane) * ROWS < q.rows) attn_key_tiles<ROWS, KEYS>(a, q, tile + lane, f, n);
-            long long inc = n;
+            const int units = (long long)(tile + lane) * ROWS < q.rows ? ITEM + n : 0;
+            long long inc = units;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -183,22 +195,23 @@ struct AttnWalk {
             const unsigned past = __ballot_sync(0xffffffffu, s.begin < item_begin + inc);
             if (past) {
                 const int l = __ffs(past) - 1;
-                tile += l, item_begin += __shfl_sync(0xffffffffu, inc - n, l);
+                tile += l, item_begin += __shfl_sync(0xffffffffu, inc - units, l);
                 first = __shfl_sync(0xffffffffu, f, l), count = __shfl_sync(0xffffffffu, n, l);
                 break;
             }
             item_begin += __shfl_sync(0xffffffffu, inc, 31);
         }
-        clip(s);
+        return clip(s) || next(a, s);
     }
-    __device__ __forceinline__ void clip(const AttnStart &s) {
-        from = (int)max(0LL, s.begin - item_begin);
-        to = (int)min((long long)count, s.end - item_begin);
+    __device__ __forceinline__ bool clip(const AttnStart &s) {
+        from = (int)max(0LL, s.begin - item_begin - ITEM);
+        to = (int)min((long long)count, s.end - item_begin - ITEM);
+        return from < to;
     }
     // The next item; false when the block's tiles are done.
     __device__ __forceinline__ bool next(const AttnArgs &a, const AttnStart &s) {
-        item_begin += count;
-        if (item_begin >= s.end) return false;
+        if (item_begin + ITEM + count >= s.end) return false;
+        item_begin += ITEM + count;
         ++tile;
         if ((long long)tile * ROWS >= q.rows) {
             tile = 0;
@@ -210,8 +223,7 @@ struct AttnWalk {
             }
         }
         attn_key_tiles<ROWS, KEYS>(a, q, tile, first, count);
-        clip(s);
-        return true;
+        return clip(s);  // only the block's last item can be without key tiles of it
     }
     __device__ __forceinline__ bool whole() const { return from == 0 && to == count; }
 };

@@ -8,6 +8,7 @@
 //   * warps 9 and 10 issue the tcgen05.mma of one row tile each: S = Q K^T into tensor memory (fp32), and O += P V with P read from tensor memory, where
 //     it overlies S.  Each row tile has two score buffers: the product of key tile n + 2 follows that of P(n) V, so that
 //     the scores of tile n + 1 are there when the softmax is done with tile n and never waits in the steady state;
+//   * warp 11 fetches the query rows;
 //   * warps 0-3 and 4-7 hold the softmax of one 128-row tile each, a row per thread: S from tensor memory, the running
 //     maximum and sum in registers, P back as 16-bit values.  O stays in tensor memory; it is rescaled only when a row's
 //     maximum has grown by more than 2^8 since its reference was set (P then reaches 256 at most, well inside fp16, and
@@ -28,8 +29,10 @@ TB200_TU_STATUS(attention_tc)
 namespace tb200 {
 
 // Of every TC_POLY_OF pairs of probabilities, TC_POLY are computed on the FP32 pipe instead of the special-function unit.
-constexpr int TC_POLY = 1, TC_POLY_OF = 4;
-constexpr int TC_ROWS = 256, TC_KEYS = 64, TC_THREADS = 384;  // three warpgroups; the last one's warps 8 to 10 work
+constexpr int TC_POLY = 1, TC_POLY_OF = 8;
+// An item costs its block about as much beside its key tiles (edge tiles, the rows' store) as this many of them.
+constexpr int TC_ITEM = 4;
+constexpr int TC_ROWS = 256, TC_KEYS = 64, TC_THREADS = 384;  // three warpgroups
 // Registers: 384 threads are launched with 168 each, which the softmax threads (64 scores and 32 words of P in registers) outgrow, so the
 // warpgroups share them anew: 2 * 192 + 120 = 3 * 168.
 constexpr int TC_SOFTMAX_REGS = 192, TC_OTHER_REGS = 120;
@@ -40,7 +43,7 @@ struct TcShape {
     static constexpr int PANELS = DPAD / 64;  // 64 columns = 128 bytes: the swizzled rows of a tile
     static constexpr int KV_PANEL = TC_KEYS * 128, KV_BYTES = PANELS * KV_PANEL;   // K or V tile
     static constexpr int Q_PANEL = 128 * 128, Q_BYTES = PANELS * Q_PANEL;          // 128 query rows
-    static constexpr int SLOTS = DPAD == 128 ? 5 : 10;                             // of K and of V
+    static constexpr int SLOTS = DPAD == 128 ? 5 : 10;                             // each a K and a V tile
     static constexpr int SMEM = 2 * Q_BYTES + 2 * SLOTS * KV_BYTES + 1024;
     static constexpr int GRID = 148;
     static constexpr size_t PART_FLOATS = (size_t)TC_ROWS * (DPAD + 2);
@@ -110,8 +113,8 @@ __device__ __forceinline__ uint32_t tc_finite_only(uint32_t w, __nv_bfloat16) {
 }
 
 struct TcShared {
-    uint64_t k_full[10], k_empty[10], v_full[10], v_empty[10];
-    uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drained[2];  // [row tile][score buffer]
+    uint64_t kv_full[10], kv_empty[10];
+    uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drained[2];  // [row tile][score buffer]
     AttnStart start;
     long long scan[32];
     uint32_t tmem_base;
@@ -120,10 +123,24 @@ struct TcShared {
     uint32_t holes[16];    // per key tile (a ring): pages of the tile that are none of the cache's
 };
 
+// Eight 16-bit values; `phase`: an address that dst differs from by a multiple of 16 bytes.
+template <class T>
+__device__ __forceinline__ void tc_store8(T *dst, const uint32_t (&h)[4], uintptr_t phase) {
+    if ((phase & 15) == 0) {
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+    } else if ((phase & 3) == 0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint32_t *>(dst + 2 * k) = h[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) reinterpret_cast<uint16_t *>(dst)[2 * k] = (uint16_t)h[k], reinterpret_cast<uint16_t *>(dst)[2 * k + 1] = (uint16_t)(h[k] >> 16);
+    }
+}
+
 // What the rows of an item see.
 struct TcItem {
     int row0, rows, base, pos_first, pos_last, key_lo, key_hi, tile0, ntiles;
-    __device__ __forceinline__ TcItem(const AttnArgs &a, const AttnWalk<TC_ROWS, TC_KEYS> &w) {
+    __device__ __forceinline__ TcItem(const AttnArgs &a, const AttnWalk<TC_ROWS, TC_KEYS, TC_ITEM> &w) {
         row0 = w.tile * TC_ROWS, rows = min(TC_ROWS, w.q.rows - row0), base = w.q.kv_len - w.q.new_tokens;
         pos_first = base + row0 / a.group, pos_last = base + (row0 + rows - 1) / a.group;
         key_lo = a.window > 0 ? max(0, pos_first - a.window + 1) : 0, key_hi = min(pos_last, w.q.visible - 1);
@@ -140,20 +157,20 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     extern __shared__ __align__(128) unsigned char tc_smem[];
     __shared__ __align__(16) TcShared sh;
     unsigned char *q_s = reinterpret_cast<unsigned char *>(((uintptr_t)tc_smem + 1023) & ~(uintptr_t)1023);  // swizzled tiles: 1024-byte bases
-    unsigned char *k_s = q_s + 2 * S::Q_BYTES, *v_s = k_s + SLOTS * S::KV_BYTES;
+    unsigned char *kv_s = q_s + 2 * S::Q_BYTES;  // slot: K tile, V tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         sh.abort_flag = 0, sh.odd_values = 0;
-        for (int i = 0; i < SLOTS; ++i) mbar_init(&sh.k_full[i], 1), mbar_init(&sh.k_empty[i], 2), mbar_init(&sh.v_full[i], 1), mbar_init(&sh.v_empty[i], 2);
+        for (int i = 0; i < SLOTS; ++i) mbar_init(&sh.kv_full[i], 1), mbar_init(&sh.kv_empty[i], 2);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.q_full[i], 128), mbar_init(&sh.pv_done[i], 1), mbar_init(&sh.o_full[i], 1), mbar_init(&sh.drained[i], 1);
+            mbar_init(&sh.q_full[i], 1), mbar_init(&sh.q_empty[i], 1), mbar_init(&sh.pv_done[i], 1), mbar_init(&sh.o_full[i], 1), mbar_init(&sh.drained[i], 1);
             for (int b = 0; b < 2; ++b) mbar_init(&sh.s_full[i][b], 1), mbar_init(&sh.p_full[i][b], 4);
         }
         mbar_fence_init();
     }
     if (warp == 8 && lane == 0) tma_prefetch_map(&map_k), tma_prefetch_map(&map_v);
-    attn_find_start<TC_THREADS, TC_ROWS, TC_KEYS>(a, &sh.start, sh.scan);
+    attn_find_start<TC_THREADS, TC_ROWS, TC_KEYS, TC_ITEM>(a, &sh.start, sh.scan);
     if (sh.start.begin >= sh.start.end) {
         if (threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
         pdl_launch_dependents();
@@ -168,9 +185,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     tc_fence_after();
     const uint32_t tmem = sh.tmem_base;
     volatile int *abortp = &sh.abort_flag;
-    AttnWalk<TC_ROWS, TC_KEYS> w;
-    w.seek(a, sh.start);
-    bool more = true, ok = true;
+    AttnWalk<TC_ROWS, TC_KEYS, TC_ITEM> w;
+    bool more = w.seek(a, sh.start), ok = true;
+    if (!more && threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
 
     if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_OTHER_REGS));
@@ -178,20 +195,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         // ---------------- producer ----------------
         const int box_keys = min(a.page_size, TC_KEYS), boxes = TC_KEYS / box_keys;
         const int behind = a.num_pages * a.kv_heads * a.page_size;  // first row behind the cache: zeros
-        uint32_t nk = 0, nv = 0;
-        // one tile: a box per page and panel, from the row that the box's lane has looked up
-        auto fetch = [&](const CUtensorMap *map, unsigned char *ring, uint64_t *full, uint64_t *empty, uint32_t &n, int row) {
-            const int s = n % SLOTS;
-            const uint32_t use = n / SLOTS;
-            if (use > 0 && !__all_sync(0xffffffffu, mbar_wait_abortable(&empty[s], (use - 1) & 1, abortp))) return false;
-            if (lane == 0) mbar_expect_tx(&full[s], S::KV_BYTES);
-            __syncwarp();
-            const int y = __shfl_sync(0xffffffffu, row, lane / PANELS);
-            if (lane < boxes * PANELS)
-                tma_load_2d(ring + s * S::KV_BYTES + (lane % PANELS) * S::KV_PANEL + (lane / PANELS) * box_keys * 128, map, (lane % PANELS) * 64, y, &full[s]);
-            ++n;
-            return true;
-        };
+        uint32_t nslot = 0, nkv = 0;
         while (more && ok) {
             const TcItem t(a, w);
             const int32_t *table = a.block_table + (long long)w.request * a.max_pages;
@@ -204,61 +208,68 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 hole = page < 0 || page >= a.num_pages;
                 return hole ? behind : (page * a.kv_heads + w.head) * a.page_size + (key - (index << a.page_shift));
             };
-            // order of use: K(0), K(1), V(0), K(2), V(1), ...
-            bool hole[3];
-            int row[3];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) row[i] = look_up(i, hole[i]);
-            auto fetch_k = [&](int r, bool h) {
-                const uint32_t holes = __ballot_sync(0xffffffffu, h);
-                if (lane == 0) sh.holes[nk & 15] = holes;
-                return fetch(&map_k, k_s, sh.k_full, sh.k_empty, nk, r);
+            // a box per page and panel, from the row that the box's lane has looked up (boxes * PANELS <= 16 lanes)
+            auto fetch = [&](const CUtensorMap *map, unsigned char *tile, uint64_t *full, int row) {
+                const int y = __shfl_sync(0xffffffffu, row, lane / PANELS);
+                if (lane < boxes * PANELS)
+                    tma_load_2d(tile + (lane % PANELS) * S::KV_PANEL + (lane / PANELS) * box_keys * 128, map, (lane % PANELS) * 64, y, full);
             };
-            ok = fetch_k(row[0], hole[0]) && (t.ntiles < 2 || fetch_k(row[1], hole[1]));
+            // slots in order of use: K(0) | K(1) | V(0), K(2) | V(1), K(3) | ... | V(last)
+            const int lead = min(2, t.ntiles);
+            bool hole = false, next_hole;
+            int row = look_up(0, hole), row1 = behind, row2 = behind;  // rows of tiles i, i - 1, i - 2
 #pragma unroll 1
-            for (int n = 0; n < t.ntiles && ok; ++n) {
-                row[2] = look_up(n + 2, hole[2]);
-                ok = fetch(&map_v, v_s, sh.v_full, sh.v_empty, nv, row[0]);
-                if (ok && n + 2 < t.ntiles) ok = fetch_k(row[2], hole[2]);
-                row[0] = row[1], row[1] = row[2];
+            for (int i = 0; i < t.ntiles + lead; ++i, ++nslot) {
+                const int next_row = look_up(i + 1, next_hole);
+                const int s = nslot % SLOTS;
+                const uint32_t use = nslot / SLOTS;
+                if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.kv_empty[s], (use - 1) & 1, abortp));
+                if (!ok) break;
+                const bool has_k = i < t.ntiles, has_v = i >= lead;
+                unsigned char *slot = kv_s + s * 2 * S::KV_BYTES;
+                if (has_k) {
+                    const uint32_t holes = __ballot_sync(0xffffffffu, hole);
+                    if (lane == 0) sh.holes[nkv & 15] = holes;
+                    ++nkv;
+                }
+                if (lane == 0) mbar_expect_tx(&sh.kv_full[s], (has_k ? S::KV_BYTES : 0) + (has_v ? S::KV_BYTES : 0));
+                __syncwarp();
+                if (has_v) fetch(&map_v, slot + S::KV_BYTES, &sh.kv_full[s], lead == 2 ? row2 : row1);
+                if (has_k) fetch(&map_k, slot, &sh.kv_full[s], row);
+                row2 = row1, row1 = row, row = next_row, hole = next_hole;
             }
             more = w.next(a, sh.start);
         }
         // copies in flight when a wait has expired (in the normal course all have been waited for by their readers)
-        if (!ok && lane == 0) {
-            for (uint32_t k = nk > SLOTS ? nk - SLOTS : 0; k < nk; ++k)
-                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sh.k_full[k % SLOTS], (k / SLOTS) & 1); ++i) {
+        if (!ok && lane == 0)
+            for (uint32_t k = nslot > SLOTS ? nslot - SLOTS : 0; k < nslot; ++k)
+                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sh.kv_full[k % SLOTS], (k / SLOTS) & 1); ++i) {
                 }
-            for (uint32_t k = nv > SLOTS ? nv - SLOTS : 0; k < nv; ++k)
-                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&sh.v_full[k % SLOTS], (k / SLOTS) & 1); ++i) {
-                }
-        }
     } else if (warp <= 10) {
         // ---------------- products, a warp per row tile ----------------
-        // (Each wait of a warp costs it some 250 cycles even where nothing is left to wait for, and products are issued at
-        // the rate at which they run: with one warp for both tiles the tensor cores idled half of the time.)
-        // ----------------
-        // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.
+        // A wait costs this warp some 200 cycles even where nothing is left to wait for, a commit 75, and products are
+        // issued at the rate at which they run.  So a row tile has a warp of its own, and a step of it is two waits (the
+        // slot with V(n) and K(n + 2); P(n)), twelve products and one commit: the scores' barrier, after which the softmax
+        // also releases the slot.  The whole warp walks the loop, so that addresses stay in uniform registers; a lane issues.
         const int t = warp - 9;
         const bool leader = lane == 0;
-        uint32_t nk = 0, nv = 0, q_use = 0, g_s = 0, g_p = 0;  // key tiles of the block so far; items and score tiles (begun, used) of the row tile
-        const uint64_t q_desc = make_smem_desc(smem_u32(q_s) + t * S::Q_BYTES, 16, 1024), k_desc = make_smem_desc(smem_u32(k_s), 16, 1024);
-        const uint64_t v_desc = make_smem_desc(smem_u32(v_s), S::KV_PANEL, 1024);
+        uint32_t nslot = 0, q_use = 0, g_s = 0, g_p = 0;  // slots of the block so far; items and score tiles (begun, used) of the row tile
+        const uint64_t q_desc = make_smem_desc(smem_u32(q_s) + t * S::Q_BYTES, 16, 1024), k_desc = make_smem_desc(smem_u32(kv_s), 16, 1024);
+        const uint64_t v_desc = make_smem_desc(smem_u32(kv_s) + S::KV_BYTES, S::KV_PANEL, 1024);
         // S = Q K^T: both operands K-major, rows of 128 bytes, 16 columns = 32 bytes per instruction
         auto qk = [&](uint32_t slot) {
-            const uint64_t k = k_desc + (uint64_t)(slot * (S::KV_BYTES >> 4));
+            const uint64_t k = k_desc + (uint64_t)(slot * (2 * S::KV_BYTES >> 4));
             const uint32_t b = g_s++ & 1, d = tmem + t * 128 + b * 64;
             if (leader) {
 #pragma unroll
                 for (int i = 0; i < DPAD / 16; ++i)
                     tc_mma_f16(d, q_desc + (uint64_t)(((i / 4) * S::Q_PANEL + (i % 4) * 32) >> 4), k + (uint64_t)(((i / 4) * S::KV_PANEL + (i % 4) * 32) >> 4), idesc_qk, i > 0);
                 tc_commit(&sh.s_full[t][b]);
-                tc_commit(&sh.k_empty[slot]);
             }
         };
         // O (+)= P V: P in tensor memory (16 keys = 8 columns), V with its columns contiguous, 16 keys = 2048 bytes
         auto pv = [&](uint32_t slot, bool add) {
-            const uint64_t v = v_desc + (uint64_t)(slot * (S::KV_BYTES >> 4));
+            const uint64_t v = v_desc + (uint64_t)(slot * (2 * S::KV_BYTES >> 4));
             const uint32_t b = g_p & 1, p = tmem + t * 128 + b * 64, d = tmem + S::O_COL + t * 128;
             if (!__all_sync(0xffffffffu, mbar_wait_abortable(&sh.p_full[t][b], (g_p >> 1) & 1, abortp))) return false;
             ++g_p;
@@ -266,45 +277,41 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             if (leader) {
 #pragma unroll
                 for (int i = 0; i < TC_KEYS / 16; ++i) tc_mma_f16_ta(d, p + i * 8, v + (uint64_t)(i * 128), idesc_pv, add || i > 0);
-                tc_commit(&sh.pv_done[t]);
-                tc_commit(&sh.v_empty[slot]);
             }
             return true;
         };
-        auto wait_full = [&](uint64_t *full, uint32_t n) {
-            const bool r = __all_sync(0xffffffffu, mbar_wait_abortable(&full[n % SLOTS], (n / SLOTS) & 1, abortp));
-            tc_fence_after();
-            return r;
-        };
+        auto wait_slot = [&]() { return __all_sync(0xffffffffu, mbar_wait_abortable(&sh.kv_full[nslot % SLOTS], (nslot / SLOTS) & 1, abortp)); };
         while (more && ok) {
             const TcItem im(a, w);
-            if (t == 1 && im.rows <= 128) {  // nothing to multiply: this warp's share of the slots is released in turn
+            const int lead = min(2, im.ntiles);
+            if (t == 1 && im.rows <= 128) {  // nothing to multiply: this row tile's share of the slots is released in turn
 #pragma unroll 1
-                for (int n = 0; n < im.ntiles && ok; ++n) {
-                    ok = wait_full(sh.k_full, nk);
-                    if (ok && leader) mbar_arrive(&sh.k_empty[nk % SLOTS]);
-                    ++nk;
-                    ok = ok && wait_full(sh.v_full, nv);
-                    if (ok && leader) mbar_arrive(&sh.v_empty[nv % SLOTS]);
-                    ++nv;
+                for (int i = 0; i < im.ntiles + lead && ok; ++i, ++nslot) {
+                    ok = wait_slot();
+                    if (ok && leader) mbar_arrive(&sh.kv_empty[nslot % SLOTS]);
                 }
                 more = w.next(a, sh.start);
                 continue;
             }
             ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.q_full[t], q_use++ & 1, abortp));
 #pragma unroll 1
-            for (int n = 0; n < min(2, im.ntiles) && ok; ++n) {
-                if (!(ok = wait_full(sh.k_full, nk))) break;
-                qk(nk++ % SLOTS);
+            for (int n = 0; n < lead && ok; ++n) {
+                if (!(ok = wait_slot())) break;
+                tc_fence_after();
+                qk(nslot++ % SLOTS);
             }
+            if (ok && leader && im.ntiles <= 2) tc_commit(&sh.q_empty[t]);
 #pragma unroll 1
-            for (int n = 0; n < im.ntiles && ok; ++n) {
-                const bool next = n + 2 < im.ntiles;
-                if (!(ok = wait_full(sh.v_full, nv))) break;
-                if (next && !(ok = wait_full(sh.k_full, nk))) break;
-                if (!(ok = pv(nv++ % SLOTS, n > 0))) break;
-                if (next) qk(nk++ % SLOTS);
-                else if (n + 1 == im.ntiles && leader) tc_commit(&sh.o_full[t]);
+            for (int n = 0; n < im.ntiles && ok; ++n, ++nslot) {
+                const uint32_t slot = nslot % SLOTS;
+                if (!(ok = wait_slot())) break;
+                if (!(ok = pv(slot, n > 0))) break;
+                if (n + 2 < im.ntiles) {
+                    qk(slot);
+                    if (n + 3 == im.ntiles && leader) tc_commit(&sh.q_empty[t]);
+                } else if (leader) {
+                    tc_commit(n + 1 == im.ntiles ? &sh.o_full[t] : &sh.pv_done[t]);
+                }
             }
             more = w.next(a, sh.start);
         }
@@ -314,45 +321,68 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
         }
         __syncwarp();
+    } else {
+        // ---------------- query rows ----------------
+        // An item's rows go to shared memory by asynchronous copies as soon as the products of the item before have read
+        // theirs, which is two key tiles and an epilogue before they are needed.  DPAD / 8 lanes share a row, so that the
+        // reads are whole lines.
+        const bool q_vec = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 8 == 0;
+        const int chunks = a.head_dim / 8;
+        constexpr int CPR = DPAD / 8, STEP = 32 / CPR;
+        const int c = lane % CPR, r0 = lane / CPR, token_step = STEP / a.group, in_step = STEP - token_step * a.group;
+        uint32_t use[2] = {0, 0};
+        while (more && ok) {
+            const int item_rows = w.q.rows - w.tile * TC_ROWS;
+            const T *q = static_cast<const T *>(a.q) + w.q.first * a.q_stride + (long long)w.head * a.group * a.head_dim + c * 8;
+#pragma unroll 1
+            for (int t = 0; t < 2 && ok && item_rows > t * 128; ++t) {
+                if (use[t] > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.q_empty[t], (use[t] - 1) & 1, abortp)))) break;
+                ++use[t];
+                unsigned char *dst = q_s + t * S::Q_BYTES + (c >> 3) * S::Q_PANEL;
+                int row = w.tile * TC_ROWS + t * 128 + r0, token = row / a.group, in = row - token * a.group;  // head of the group
+                if (q_vec) {
+#pragma unroll 4
+                    for (int r = r0; r < 128; r += STEP, row += STEP) {
+                        const bool there = row < w.q.rows && c < chunks;
+                        const T *src = there ? q + token * a.q_stride + (long long)in * a.head_dim : static_cast<const T *>(a.q);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4))), "l"(src), "r"(there ? 16 : 0)
+                                     : "memory");
+                        token += token_step, in += in_step;
+                        if (in >= a.group) in -= a.group, ++token;
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                } else {
+#pragma unroll 1
+                    for (int r = r0; r < 128; r += STEP, row += STEP) {
+                        const bool there = row < w.q.rows && c < chunks;
+                        const uint16_t *src = reinterpret_cast<const uint16_t *>(q + token * a.q_stride + (long long)in * a.head_dim);
+                        uint32_t h[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) h[i] = there ? src[i] : 0;
+                        *reinterpret_cast<uint4 *>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                        token += token_step, in += in_step;
+                        if (in >= a.group) in -= a.group, ++token;
+                    }
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.q_full[t]);
+            }
+            more = w.next(a, sh.start);
+        }
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_SOFTMAX_REGS));
         // ---------------- softmax ----------------
-        const int t = warp >> 2, row_in = threadIdx.x & 127, D = a.head_dim, chunks = D / 8;
+        const int t = warp >> 2, row_in = threadIdx.x & 127, D = a.head_dim;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + S::O_COL + t * 128;
-        uint32_t nkv = 0, g = 0, o_use = 0;  // key tiles of the block so far, score tiles of this row tile, items of this row tile
-        // The next item that has rows for this tile: its query rows to shared memory by asynchronous copies (DPAD / 8
-        // threads share a row, so that the reads are whole lines).
+        uint32_t nkv = 0, nslot = 0, g = 0, o_use = 0, pv_use = 0;  // key tiles and slots of the block so far; score tiles and items of the row tile
+        // the next item that has rows for this tile
         auto take_item = [&]() {
             while (more && t == 1 && w.q.rows - w.tile * TC_ROWS <= 128) {
-                nkv += w.to - w.from;
+                nkv += w.to - w.from, nslot += w.to - w.from + min(2, w.to - w.from);
                 more = w.next(a, sh.start);
             }
-            if (!more) return;
-            constexpr int CPR = DPAD / 8, STEP = 128 / CPR;
-            const int c = row_in % CPR, r0 = row_in / CPR, row0 = w.tile * TC_ROWS + t * 128;
-            const bool q_vec = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 8 == 0;
-            const T *q = static_cast<const T *>(a.q) + w.q.first * a.q_stride + (long long)w.head * a.group * D + c * 8;
-            unsigned char *dst = q_s + t * S::Q_BYTES + (c >> 3) * S::Q_PANEL;
-            int token = (row0 + r0) / a.group, in = row0 + r0 - token * a.group;  // head of the group
-            const int token_step = STEP / a.group, in_step = STEP - token_step * a.group;
-#pragma unroll 1
-            for (int r = r0; r < 128; r += STEP) {
-                const bool there = row0 + r < w.q.rows && c < chunks;
-                const T *src = there ? q + token * a.q_stride + (long long)in * D : static_cast<const T *>(a.q);
-                token += token_step, in += in_step;
-                if (in >= a.group) in -= a.group, ++token;
-                unsigned char *at = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                if (q_vec) {
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at)), "l"(src), "r"(there ? 16 : 0) : "memory");
-                } else {
-#pragma unroll 1
-                    for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t *>(at)[i] = there ? reinterpret_cast<const uint16_t *>(src)[i] : (uint16_t)0;
-                }
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_async_shared();
-            mbar_arrive(&sh.q_full[t]);
         };
         take_item();
         while (more && ok) {
@@ -362,29 +392,39 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const int pos = have ? im.base + (im.row0 + my_row) / a.group : -1;
             const int see_hi = min(pos, w.q.visible - 1), see_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
             const uint64_t scale2 = tc_pair(a.scale_log2, a.scale_log2);
+            const int lead = min(2, im.ntiles);
+            pv_use += lead - 1;  // an item of two tiles or more commits the last product but one
             float m = -INFINITY, l = 0.0f;
-#pragma unroll 1
-            for (int n = 0; n < im.ntiles; ++n, ++nkv, ++g) {
-                const uint32_t b = g & 1;
-                ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.s_full[t][b], (g >> 1) & 1, abortp));
-                if (!ok) break;
+            uint32_t s[64];
+            const uint32_t nslot0 = nslot;
+            // The scores of tile n, and the release of the slot whose products (K(n) and V(n - 1)) are done by then.
+            auto scores_there = [&](int n) {
                 tc_fence_after();
+                if (row_in == 0) mbar_arrive(&sh.kv_empty[(nslot0 + n) % SLOTS]);
+            };
+            ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.s_full[t][g & 1], (g >> 1) & 1, abortp));
+            if (!ok) break;
+            scores_there(0);
+            if (warp_has) {
+                tc_ld_32cols(s_addr + (g & 1) * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                tc_ld_32cols(s_addr + (g & 1) * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+            }
+#pragma unroll 1
+            for (int n = 0; n < im.ntiles; ++n, ++nkv, ++nslot, ++g) {
+                const uint32_t b = g & 1;
                 const int key0 = (im.tile0 + n) * TC_KEYS;
                 const uint32_t holes = sh.holes[nkv & 15];
                 const bool edge = key0 + TC_KEYS - 1 > min(im.pos_first, im.key_hi) || (a.window > 0 && key0 <= im.pos_last - a.window);
-                uint32_t s[64];
                 float top = -INFINITY;
                 if (warp_has) {
-                    tc_ld_32cols(s_addr + b * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-                    tc_ld_32cols(s_addr + b * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
                     tc_wait_ld();
-                    if (edge) {
+                    if (__builtin_expect(edge, 0)) {
                         const int lo = see_lo - key0, hi = see_hi - key0;
 #pragma unroll
                         for (int i = 0; i < 64; ++i)
                             if (i > hi || i < lo) s[i] = 0xFF800000u;
                     }
-                    if (holes) {
+                    if (__builtin_expect(holes != 0, 0)) {
                         const int shift = min(a.page_shift, 6);
 #pragma unroll
                         for (int i = 0; i < 64; ++i)
@@ -395,15 +435,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     for (int i = 0; i < 64; i += 2) x[(i >> 1) & 3] = tc_max3(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                     top = tc_max3(tc_max3(x[0], x[1], x[2]), x[3], x[3]) * a.scale_log2;
                 }
-                if (edge) {
+                if (__builtin_expect(edge, 0)) {
                     // A place that no row sees may hold anything, and one that some rows see and others do not may hold
                     // an infinity or a NaN: 0 * V would carry it to rows that do not see it.  The former become zeros
                     // here; of the latter the values that are not finite do, and the epilogue gives them to their rows.
                     // (Both tiles' warps do so, two threads a key; they write the same.)
-                    ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.v_full[nkv % SLOTS], (nkv / SLOTS) & 1, abortp));
+                    const uint32_t vs = nslot + lead;
+                    ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.kv_full[vs % SLOTS], (vs / SLOTS) & 1, abortp));
                     if (!ok) break;
                     const int in = row_in >> 1, key = key0 + in;
-                    unsigned char *v_row = v_s + (nkv % SLOTS) * S::KV_BYTES + in * 128;
+                    unsigned char *v_row = kv_s + (vs % SLOTS) * 2 * S::KV_BYTES + S::KV_BYTES + in * 128;
                     const bool unseen = key > im.key_hi || key < im.key_lo;
                     if (unseen || key > im.pos_first || (a.window > 0 && key <= im.pos_last - a.window)) {
 #pragma unroll 1
@@ -418,12 +459,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     fence_async_shared();
                 }
+                bool ahead = false;
                 if (warp_has) {
-                    if (n == 0) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                        // the product before this one may still be adding to O
-                        ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.pv_done[t], (g - 1) & 1, abortp));
+                    if (n == 0) m = top;
+                    if (__builtin_expect(__any_sync(0xffffffffu, top > m + 8.0f), 0)) {
+                        // The product before this one may still be adding to O.  The next scores' product follows it; behind
+                        // the last scores it has a barrier of its own.
+                        ok = __all_sync(0xffffffffu, n + 1 < im.ntiles ? mbar_wait_abortable(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1, abortp)
+                                                                       : mbar_wait_abortable(&sh.pv_done[t], (pv_use - 1) & 1, abortp));
                         if (!ok) break;
                         tc_fence_after();
                         const float next = fmaxf(m, top), f = next == m ? 1.0f : tc_ex2(m - next);
@@ -440,42 +483,62 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     const float shift = m == -INFINITY ? 0.0f : -m;
                     const uint64_t shift2 = tc_pair(shift, shift);
+                    // Where the next scores are there already they are read as soon as the registers of this tile's come
+                    // free, so that the wait for them and the way from tensor memory are hidden behind the powers.
+                    const uint32_t next = s_addr + (b ^ 1) * 64;
+                    ahead = n + 1 < im.ntiles && __all_sync(0xffffffffu, mbar_try_wait(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1));
+                    if (ahead) scores_there(n + 1);
                     uint64_t sum[2] = {0, 0};
                     uint32_t p[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const uint64_t x2 = tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift2);
-                        float p0, p1;
-                        if (i % TC_POLY_OF < TC_POLY) {
-                            tc_ex2_pair(x2, p0, p1);
-                        } else {
-                            tc_split(x2, p0, p1);
-                            p0 = tc_ex2(p0), p1 = tc_ex2(p1);
+                    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                        for (int i = 16 * c; i < 16 * c + 16; ++i) {
+                            const uint64_t x2 = tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift2);
+                            float p0, p1;
+                            if (i % TC_POLY_OF < TC_POLY) {
+                                tc_ex2_pair(x2, p0, p1);
+                            } else {
+                                tc_split(x2, p0, p1);
+                                p0 = tc_ex2(p0), p1 = tc_ex2(p1);
+                            }
+                            sum[i & 1] = tc_add2(sum[i & 1], tc_pair(p0, p1));
+                            p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
                         }
-                        sum[i & 1] = tc_add2(sum[i & 1], tc_pair(p0, p1));
-                        p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
+                        if (c == 1) tc_st_32cols(s_addr + b * 64, p);
+                        if (ahead) tc_ld_32cols(next + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
                     }
-                    tc_st_32cols(s_addr + b * 64, p);
                     float s0, s1;
                     tc_split(tc_add2(sum[0], sum[1]), s0, s1);
                     l += s0 + s1;
-                    if (!(top < INFINITY)) l = __int_as_float(0x7FC00000);  // a score of +infinity or NaN: the row is NaN
+                    if (__builtin_expect(!(top < INFINITY), 0)) l = __int_as_float(0x7FC00000);  // a score of +infinity or NaN: the row is NaN
                     tc_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.p_full[t][b]);
+                if (!ahead && n + 1 < im.ntiles) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1, abortp));
+                    if (!ok) break;
+                    scores_there(n + 1);
+                    if (warp_has) {
+                        tc_ld_32cols(s_addr + (b ^ 1) * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                        tc_ld_32cols(s_addr + (b ^ 1) * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+                    }
+                }
             }
             if (!ok) break;
-            // All scores of the item have been read, so its query rows are done with: the next item's are fetched while
-            // the last products run.
-            const AttnWalk<TC_ROWS, TC_KEYS> done = w;
+            const AttnWalk<TC_ROWS, TC_KEYS, TC_ITEM> done = w;
+            const uint32_t nslot_done = nslot;  // the slots of the last products
+            nslot += lead;
             more = w.next(a, sh.start);
             const bool last = !more;
             take_item();
             ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.o_full[t], o_use++ & 1, abortp));
             if (!ok) break;
             tc_fence_after();
+            if (row_in == 0)
+                for (int i = 0; i < lead; ++i) mbar_arrive(&sh.kv_empty[(nslot_done + i) % SLOTS]);
             const bool whole = done.whole(), odd = *reinterpret_cast<volatile int *>(&sh.odd_values) != 0;
             if (warp_has) {
                 const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
@@ -506,27 +569,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                         for (int i = 0; i < 32; ++i) part[(c * 32 + i) * TC_ROWS] = __uint_as_float(o[i]);
                     } else if (have) {
-                        uint32_t h[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) h[i] = pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv, T());
                         T *d = dst + c * 32;
-                        const uintptr_t phase = (uintptr_t)d;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {  // pieces of 8 columns
                             if (c * 32 + i * 8 >= D) break;
-                            if ((phase & 15) == 0) {
-                                *reinterpret_cast<uint4 *>(d + i * 8) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-                            } else {
+                            uint32_t h[4];
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    if ((phase & 3) == 0) {
-                                        *reinterpret_cast<uint32_t *>(d + i * 8 + 2 * k) = h[4 * i + k];
-                                    } else {
-                                        reinterpret_cast<uint16_t *>(d)[i * 8 + 2 * k] = (uint16_t)h[4 * i + k];
-                                        reinterpret_cast<uint16_t *>(d)[i * 8 + 2 * k + 1] = (uint16_t)(h[4 * i + k] >> 16);
-                                    }
-                                }
-                            }
+                            for (int k = 0; k < 4; ++k) h[k] = pack2(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv, T());
+                            tc_store8(d + i * 8, h, (uintptr_t)d);
                         }
                     }
                 }
@@ -534,7 +584,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             if (threadIdx.x == 0) {
                 if (!whole && done.from == 0)
-                    a.joins[blockIdx.x] = make_int4(done.request, done.head, done.tile, attn_block_of(sh.start.total, sh.start.blocks, done.item_begin + done.count - 1));
+                    a.joins[blockIdx.x] = make_int4(done.request, done.head, done.tile, attn_block_of(sh.start.total, sh.start.blocks, done.item_begin + TC_ITEM + done.count - 1));
                 else if (last)
                     a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
             }
@@ -578,9 +628,15 @@ __global__ void __launch_bounds__(DPAD * 2) attn_tc_join_kernel(AttnArgs a) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int at = item.z * TC_ROWS + row, token = at / a.group, head = item.y * a.group + at % a.group;
     T *dst = static_cast<T *>(a.out) + (q.first + token) * a.out_stride + (long long)head * a.head_dim + d0;
+    const uintptr_t phase = (uintptr_t)dst;
 #pragma unroll
-    for (int c = 0; c < 16; ++c)
-        if (d0 + c < a.head_dim) from_f32(dst[c], acc[c] * inv);
+    for (int c = 0; c < 16; c += 8) {  // whole sectors where the alignment allows it
+        if (d0 + c >= a.head_dim) break;
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = pack2(acc[c + 2 * i] * inv, acc[c + 2 * i + 1] * inv, T());
+        tc_store8(dst + c, h, phase);
+    }
 }
 
 // ---------------------------------------------------------------------------
