@@ -28,8 +28,6 @@ TB200_TU_STATUS(attention_tc)
 
 namespace tb200 {
 
-// Of every TC_POLY_OF pairs of probabilities, TC_POLY are computed on the FP32 pipe instead of the special-function unit.
-constexpr int TC_POLY = 1, TC_POLY_OF = 8;
 // An item costs its block about as much beside its key tiles (edge tiles, the rows' store) as this many of them.
 constexpr int TC_ITEM = 4;
 constexpr int TC_ROWS = 256, TC_KEYS = 64, TC_THREADS = 384;  // three warpgroups
@@ -69,26 +67,17 @@ __device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^x on the FP32 pipe, for x <= 16; the special-function unit gives 16 powers a cycle and SM, which alone would take as
-// long as both products of a tile.  x = n + f with n = round(x) (by adding 1.5 * 2^23), |f| <= 1/2; 2^f is a polynomial
-// of degree 4 with p(0) = 1, fitted to the smallest largest relative error (2.9e-6, below the rounding of P by a factor
-// of 80 at least); n goes into the exponent.  x is held at -127, where the sum of exponents is that of zero: masked
-// scores give 0.
-__device__ __forceinline__ void tc_ex2_pair(uint64_t x2, float &p0, float &p1) {
-    float x, y;
-    tc_split(x2, x, y);
-    x2 = tc_pair(fmaxf(x, -127.0f), fmaxf(y, -127.0f));
-    const uint64_t n2 = tc_add2(x2, tc_pair(12582912.0f, 12582912.0f));
-    const uint64_t f2 = tc_fma2(tc_add2(n2, tc_pair(-12582912.0f, -12582912.0f)), tc_pair(-1.0f, -1.0f), x2);
-    uint64_t p2 = tc_fma2(f2, tc_pair(0.009582853f, 0.009582853f), tc_pair(0.055906426f, 0.055906426f));
-    p2 = tc_fma2(p2, f2, tc_pair(0.24024099f, 0.24024099f));
-    p2 = tc_fma2(p2, f2, tc_pair(0.69312418f, 0.69312418f));
-    p2 = tc_fma2(p2, f2, tc_pair(1.0f, 1.0f));
-    float n0, n1;
-    tc_split(n2, n0, n1);
-    tc_split(p2, p0, p1);
-    p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
-    p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
+// Whether the phase is over, without the wait that try_wait may put in front of its answer.
+__device__ __forceinline__ bool tc_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 // the largest of three, NaN if one of them is
 __device__ __forceinline__ float tc_max3(float a, float b, float c) {
@@ -486,7 +475,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     // Where the next scores are there already they are read as soon as the registers of this tile's come
                     // free, so that the wait for them and the way from tensor memory are hidden behind the powers.
                     const uint32_t next = s_addr + (b ^ 1) * 64;
-                    ahead = n + 1 < im.ntiles && __all_sync(0xffffffffu, mbar_try_wait(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1));
+                    ahead = n + 1 < im.ntiles && __all_sync(0xffffffffu, tc_test(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1));
                     if (ahead) scores_there(n + 1);
                     uint64_t sum[2] = {0, 0};
                     uint32_t p[32];
@@ -496,12 +485,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         for (int i = 16 * c; i < 16 * c + 16; ++i) {
                             const uint64_t x2 = tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift2);
                             float p0, p1;
-                            if (i % TC_POLY_OF < TC_POLY) {
-                                tc_ex2_pair(x2, p0, p1);
-                            } else {
-                                tc_split(x2, p0, p1);
-                                p0 = tc_ex2(p0), p1 = tc_ex2(p1);
-                            }
+                            tc_split(x2, p0, p1);
+                            p0 = tc_ex2(p0), p1 = tc_ex2(p1);
                             sum[i & 1] = tc_add2(sum[i & 1], tc_pair(p0, p1));
                             p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
                         }
