@@ -29,7 +29,7 @@ TB200_TU_STATUS(attention_tc)
 namespace tb200 {
 
 // An item costs its block about as much beside its key tiles (edge tiles, the rows' store) as this many of them.
-constexpr int TC_ITEM = 4;
+constexpr int TC_ITEM = 8;
 constexpr int TC_ROWS = 256, TC_KEYS = 64, TC_THREADS = 384;  // three warpgroups
 // Registers: 384 threads are launched with 168 each, which the softmax threads (64 scores and 32 words of P in registers) outgrow, so the
 // warpgroups share them anew: 2 * 192 + 120 = 3 * 168.
@@ -66,18 +66,6 @@ __device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
-}
-// Whether the phase is over, without the wait that try_wait may put in front of its answer.
-__device__ __forceinline__ bool tc_test(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
 }
 // the largest of three, NaN if one of them is
 __device__ __forceinline__ float tc_max3(float a, float b, float c) {
@@ -384,28 +372,21 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const int lead = min(2, im.ntiles);
             pv_use += lead - 1;  // an item of two tiles or more commits the last product but one
             float m = -INFINITY, l = 0.0f;
-            uint32_t s[64];
-            const uint32_t nslot0 = nslot;
-            // The scores of tile n, and the release of the slot whose products (K(n) and V(n - 1)) are done by then.
-            auto scores_there = [&](int n) {
-                tc_fence_after();
-                if (row_in == 0) mbar_arrive(&sh.kv_empty[(nslot0 + n) % SLOTS]);
-            };
-            ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.s_full[t][g & 1], (g >> 1) & 1, abortp));
-            if (!ok) break;
-            scores_there(0);
-            if (warp_has) {
-                tc_ld_32cols(s_addr + (g & 1) * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-                tc_ld_32cols(s_addr + (g & 1) * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
-            }
 #pragma unroll 1
             for (int n = 0; n < im.ntiles; ++n, ++nkv, ++nslot, ++g) {
                 const uint32_t b = g & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.s_full[t][b], (g >> 1) & 1, abortp));
+                if (!ok) break;
+                tc_fence_after();
+                if (row_in == 0) mbar_arrive(&sh.kv_empty[nslot % SLOTS]);  // the products that read K(n) and V(n - 2) are done
                 const int key0 = (im.tile0 + n) * TC_KEYS;
                 const uint32_t holes = sh.holes[nkv & 15];
                 const bool edge = key0 + TC_KEYS - 1 > min(im.pos_first, im.key_hi) || (a.window > 0 && key0 <= im.pos_last - a.window);
+                uint32_t s[64];
                 float top = -INFINITY;
                 if (warp_has) {
+                    tc_ld_32cols(s_addr + b * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                    tc_ld_32cols(s_addr + b * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
                     tc_wait_ld();
                     if (__builtin_expect(edge, 0)) {
                         const int lo = see_lo - key0, hi = see_hi - key0;
@@ -448,7 +429,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     fence_async_shared();
                 }
-                bool ahead = false;
                 if (warp_has) {
                     if (n == 0) m = top;
                     if (__builtin_expect(__any_sync(0xffffffffu, top > m + 8.0f), 0)) {
@@ -472,27 +452,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     const float shift = m == -INFINITY ? 0.0f : -m;
                     const uint64_t shift2 = tc_pair(shift, shift);
-                    // Where the next scores are there already they are read as soon as the registers of this tile's come
-                    // free, so that the wait for them and the way from tensor memory are hidden behind the powers.
-                    const uint32_t next = s_addr + (b ^ 1) * 64;
-                    ahead = n + 1 < im.ntiles && __all_sync(0xffffffffu, tc_test(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1));
-                    if (ahead) scores_there(n + 1);
                     uint64_t sum[2] = {0, 0};
                     uint32_t p[32];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                        for (int i = 16 * c; i < 16 * c + 16; ++i) {
-                            const uint64_t x2 = tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift2);
-                            float p0, p1;
-                            tc_split(x2, p0, p1);
-                            p0 = tc_ex2(p0), p1 = tc_ex2(p1);
-                            sum[i & 1] = tc_add2(sum[i & 1], tc_pair(p0, p1));
-                            p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
-                        }
-                        if (c == 1) tc_st_32cols(s_addr + b * 64, p);
-                        if (ahead) tc_ld_32cols(next + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+                    for (int i = 0; i < 32; ++i) {
+                        float p0, p1;
+                        tc_split(tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift2), p0, p1);
+                        p0 = tc_ex2(p0), p1 = tc_ex2(p1);
+                        sum[i & 1] = tc_add2(sum[i & 1], tc_pair(p0, p1));
+                        p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
                     }
+                    tc_st_32cols(s_addr + b * 64, p);
                     float s0, s1;
                     tc_split(tc_add2(sum[0], sum[1]), s0, s1);
                     l += s0 + s1;
@@ -502,15 +472,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.p_full[t][b]);
-                if (!ahead && n + 1 < im.ntiles) {
-                    ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1, abortp));
-                    if (!ok) break;
-                    scores_there(n + 1);
-                    if (warp_has) {
-                        tc_ld_32cols(s_addr + (b ^ 1) * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-                        tc_ld_32cols(s_addr + (b ^ 1) * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
-                    }
-                }
             }
             if (!ok) break;
             const AttnWalk<TC_ROWS, TC_KEYS, TC_ITEM> done = w;
