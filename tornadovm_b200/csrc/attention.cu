@@ -5,7 +5,7 @@
 //     m' = max(m, max_j s_j),  p_j = 2^(s_j - m'),  l' = l 2^(m - m') + sum p_j,  O' = O 2^(m - m') + p V
 //
 // A decoding request reads its whole cache for `group` rows: bound by memory, floor = the bytes of K and V.  So the key
-// tiles of all requests are divided evenly over the resident blocks (attention.cuh), each of which keeps two to three
+// tiles of all requests are divided evenly over the resident blocks (attention.cuh), each of which keeps one to three
 // tiles of 64 keys in flight with 16-byte asynchronous copies; a page may have any size, since every row of a tile is
 // fetched through its own table entry, looked up two tiles ahead.  Rows that no query row of the tile sees are filled
 // with zeros and not read.  The products run as mma.sync.m16n8k16 with fp32 accumulators: with up to 16 rows the four
@@ -59,8 +59,11 @@ __device__ __forceinline__ void at_mma(float (&d)[4], const uint32_t (&a)[4], ui
 template <int DPAD, bool SPLIT_KEYS>
 struct AtShape {
     static constexpr int ROWS = SPLIT_KEYS ? 16 : 64;
-    static constexpr int STAGES = DPAD == 64 ? 4 : SPLIT_KEYS ? 3 : 2;  // two blocks an SM up to 128 columns
-    static constexpr int BLOCKS_PER_SM = DPAD == 256 ? 1 : 2;
+    // The copies in flight hide the memory's latency, several blocks an SM each other's arithmetic: with 128 columns three
+    // blocks of two stages read 64 requests of up to 8192 keys in 196 us, two of three in 230 us or more; with 64 columns
+    // four blocks of three stages in 113 us, three of four in 127 us.
+    static constexpr int STAGES = DPAD == 64 ? (SPLIT_KEYS ? 3 : 4) : DPAD == 128 ? 2 : SPLIT_KEYS ? 3 : 2;
+    static constexpr int BLOCKS_PER_SM = DPAD == 256 ? 1 : !SPLIT_KEYS ? 2 : DPAD == 64 ? 4 : 3;
     static constexpr int ROW_BYTES = DPAD * 2, TILE_BYTES = AT_KEYS * ROW_BYTES, Q_BYTES = ROWS * ROW_BYTES;
     static constexpr int RING = STAGES + 1;  // tiles whose rows have been looked up
     static constexpr int SMEM = Q_BYTES + STAGES * 2 * TILE_BYTES + RING * AT_KEYS * 8 + RING * 2 * 4;
@@ -82,13 +85,14 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
     constexpr bool Q_IN_REGS = DPAD <= 128;
     extern __shared__ __align__(1024) unsigned char at_smem[];
     unsigned char *q_s = at_smem, *kv_s = at_smem + S::Q_BYTES;
-    long long *row_s = reinterpret_cast<long long *>(kv_s + STAGES * 2 * TILE_BYTES);  // [RING][64]: row of the cache, -1: none
+    long long *row_s = reinterpret_cast<long long *>(kv_s + STAGES * 2 * TILE_BYTES);  // [RING][64]: place in the cache, -1: none
     int *hole_s = reinterpret_cast<int *>(row_s + RING * AT_KEYS);                     // [RING][2]: a row of the tile's half is missing
     __shared__ AttnStart start;
     __shared__ long long scan[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int D = a.head_dim, ksteps = (D + 15) / 16, dchunks = D / 8, lchunks = 2 * ksteps;
     const int warp_key = SPLIT_KEYS ? warp * 16 : 0, warp_row = SPLIT_KEYS ? 0 : warp * 16;
+    const long long v_ahead = static_cast<const char *>(a.v_cache) - static_cast<const char *>(a.k_cache);
     const bool copy16 = ((uintptr_t)a.k_cache & 15) == 0 && ((uintptr_t)a.v_cache & 15) == 0;
 
     attn_find_start<AT_THREADS, ROWS, AT_KEYS, AT_ITEM>(a, &start, scan);
@@ -109,35 +113,41 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
         const int tile0 = w.first + w.from, ntiles = w.to - w.from;
         const int32_t *table = a.block_table + (long long)w.request * a.max_pages;
 
-        // row of the cache that holds key `key` of the request for this head
+        // where in the cache key `key` of the request lies for this head, in bytes
         auto look_up = [&](int key) -> long long {
             if (key < key_lo || key > key_hi) return -1;
             const int index = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
             const int page = table[index];
             if (page < 0 || page >= a.num_pages) return -1;
-            return ((long long)page * a.kv_heads + w.head) * a.page_size + (key - index * a.page_size);
+            return (((long long)page * a.kv_heads + w.head) * a.page_size + (key - index * a.page_size)) * (2 * D);
         };
         auto put_row = [&](int slot, long long row) {  // warps 0 and 1
             row_s[slot * AT_KEYS + tid] = row;
             const bool hole = __any_sync(0xffffffffu, row < 0);
             if (lane == 0) hole_s[slot * 2 + warp] = hole;
         };
+        // a thread copies one 16-byte column of every RSTEP-th row
         auto load_tile = [&](int i) {
-            unsigned char *ks = kv_s + (i % STAGES) * 2 * TILE_BYTES, *vs = ks + TILE_BYTES;
+            constexpr int CHUNKS = DPAD / 8, RSTEP = AT_THREADS / CHUNKS;
+            const int chunk = tid % CHUNKS, r0 = tid / CHUNKS;
+            if (chunk >= lchunks) return;
+            const uint32_t ks = smem_u32(kv_s) + (i % STAGES) * 2 * TILE_BYTES;
             const long long *rows_of = row_s + (i % RING) * AT_KEYS;
-            for (int e = tid; e < AT_KEYS * lchunks; e += AT_THREADS) {
-                const int row = e / lchunks, chunk = e - row * lchunks;
-                const long long src_row = rows_of[row];
-                const int bytes = src_row >= 0 && chunk < dchunks ? 16 : 0;
-                const long long at = bytes ? src_row * D + chunk * 8 : 0;
-                const uint32_t off = at_swizzle<DPAD>(row, chunk);
-                const T *k = static_cast<const T *>(a.k_cache) + at, *v = static_cast<const T *>(a.v_cache) + at;
+            const char *column = static_cast<const char *>(a.k_cache) + chunk * 16;
+#pragma unroll
+            for (int n = 0; n < AT_KEYS / RSTEP; ++n) {
+                const int row = r0 + n * RSTEP;
+                const long long at = rows_of[row];
+                const bool there = at >= 0 && chunk < dchunks;
+                const char *k = there ? column + at : static_cast<const char *>(a.k_cache);
+                const uint32_t dst = ks + at_swizzle<DPAD>(row, chunk);
                 if (copy16) {
-                    at_copy16(smem_u32(ks + off), k, bytes);
-                    at_copy16(smem_u32(vs + off), v, bytes);
+                    at_copy16(dst, k, there ? 16 : 0);
+                    at_copy16(dst + TILE_BYTES, k + v_ahead, there ? 16 : 0);
                 } else {
-                    at_copy8(smem_u32(ks + off), k, bytes / 2), at_copy8(smem_u32(ks + off + 8), k + (bytes ? 4 : 0), bytes / 2);
-                    at_copy8(smem_u32(vs + off), v, bytes / 2), at_copy8(smem_u32(vs + off + 8), v + (bytes ? 4 : 0), bytes / 2);
+                    const int step = there ? 8 : 0;
+                    at_copy8(dst, k, step), at_copy8(dst + 8, k + step, step);
+                    at_copy8(dst + TILE_BYTES, k + v_ahead, step), at_copy8(dst + TILE_BYTES + 8, k + v_ahead + step, step);
                 }
             }
         };

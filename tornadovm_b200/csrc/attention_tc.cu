@@ -67,13 +67,6 @@ __device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// the largest of three, NaN if one of them is
-__device__ __forceinline__ float tc_max3(float a, float b, float c) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 __device__ __forceinline__ float tc_ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -402,8 +395,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) x[(i >> 1) & 3] = tc_max3(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                    top = tc_max3(tc_max3(x[0], x[1], x[2]), x[3], x[3]) * a.scale_log2;
+                    for (int i = 0; i < 64; i += 2) x[(i >> 1) & 3] = max3_nan(x[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                    top = max3_nan(max3_nan(x[0], x[1], x[2]), x[3], x[3]) * a.scale_log2;
                 }
                 if (__builtin_expect(edge, 0)) {
                     // A place that no row sees may hold anything, and one that some rows see and others do not may hold

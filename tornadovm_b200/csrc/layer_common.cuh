@@ -104,4 +104,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 }  // namespace tb200

@@ -8,11 +8,15 @@
 // The norm is that of the unrounded fp32 sum h: residual_out's rounding is the only one before q.
 //
 // Bound by memory: x, residual, residual_out and q are each touched once (7 bytes an element for 16-bit arrays).  A
-// row lives in the registers of one block between the two reductions (sum of squares; the largest |y| of a group is a
-// shuffle among the 4, 8 or 16 lanes that hold it, or a second block reduction for a scale a row), so nothing is read
-// twice; rows that outgrow the registers (above 32768 columns) are read again instead.  A thread holds eight
-// consecutive columns per 16-byte load, blocks are as wide as one such load of a row needs, and a grid of resident
-// blocks walks the rows, which keeps the weight of rows of up to 8192 columns in registers.
+// row lives in the registers of one block across its reduction, so nothing is read twice.  The norm is one factor r for
+// the whole row, so max |y| = r max |h * weight|: the sum of squares and the largest |h * weight| of a row are reduced
+// together, behind one barrier, and a value costs one product with r / scale; the largest of a group is a shuffle among
+// the 4, 8 or 16 lanes that hold it.  Rows that outgrow the registers (above 32768 columns) are read again instead.
+//
+// A thread holds eight consecutive columns per 16-byte load.  Few rows are a matter of latency: a thread for each eight
+// columns.  Many rows are one of instructions and of bytes in flight: a thread for 16 columns, and the next two rows of a
+// block on their way to shared memory while it works on one (8192 x 4096 bf16 to e4m3: 47 us, 75 us with a thread for
+// each eight columns and no rows ahead).
 #include <cuda_fp8.h>
 
 #define TB200_OP_CLASS TB200_PREPARE_LAYER
@@ -30,8 +34,8 @@ struct NormArgs {
     uint8_t *q;
     float *scales;
     long long x_stride;
-    float eps;
-    int rows, cols, group, groups, format;
+    float eps, inv_cols;
+    int rows, cols, group, group_shift, groups, format;
 };
 
 __device__ __forceinline__ float format_top(int format) { return format == TB200_Q_INT8 ? 127.0f : format == TB200_Q_E4M3 ? 448.0f : 57344.0f; }
@@ -46,34 +50,44 @@ __device__ __forceinline__ float group_scale(float top_y, int format, float &inv
     return finite ? scale : top_y;
 }
 
-__device__ __forceinline__ uint32_t to_8bit(float y, float inv, int format) {
-    if (inv == 0.0f) return 0;
-    const float v = __fmul_rn(y, inv);
-    if (format == TB200_Q_INT8)  // floor(v + 1/2) in the low byte of the sum with 1.5 * 2^23, rounded down
-        return (uint32_t)__float_as_int(__fadd_rd(__fadd_rn(v, 0.5f), 12582912.0f)) & 0xFFu;
-    return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, format == TB200_Q_E4M3 ? __NV_E4M3 : __NV_E5M2);
+// Eight values of h * weight, times the norm's factor over the scale, as eight bytes; inv 0: a group that is not finite.
+__device__ __forceinline__ uint2 to_8bit(const float (&y)[8], float inv, float factor, int format) {
+    if (inv == 0.0f) return make_uint2(0, 0);
+    uint32_t w[2];
+    if (format == TB200_Q_INT8) {  // floor(v + 1/2) in the low byte of the sum with 1.5 * 2^23, rounded down
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = (uint32_t)__float_as_int(__fadd_rd(__fadd_rn(__fmul_rn(y[4 * h + j], factor), 0.5f), 12582912.0f));
+            w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float2 lo = make_float2(__fmul_rn(y[4 * h], factor), __fmul_rn(y[4 * h + 1], factor)), hi = make_float2(__fmul_rn(y[4 * h + 2], factor), __fmul_rn(y[4 * h + 3], factor));
+            if (format == TB200_Q_E4M3)
+                w[h] = __nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
+            else
+                w[h] = __nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E5M2) | (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E5M2) << 16;
+        }
+    }
+    return make_uint2(w[0], w[1]);
 }
 
-// Block reduction of one value; every thread gets the result.  `red`: 33 floats, used by one reduction at a time.
-template <bool MAX>
-__device__ __forceinline__ float block_reduce(float v, float *red) {
+// The sum of one value and the largest of another one over the block; every thread gets both.  `red`: 32 pairs that the
+// reductions before and behind this one do not use, so that one barrier is enough.
+__device__ __forceinline__ void block_reduce(float &sum, float &top, float2 *red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = MAX ? max_nan(v, w) : v + w;
-    }
-    if (warps == 1) return v;
-    __syncthreads();  // the last reduction's result has been read
-    if (lane == 0) red[warp] = v;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (warps == 1) return;
+    if (lane == 0) red[warp] = make_float2(sum, top);
     __syncthreads();
-    v = lane < warps ? red[lane] : 0.0f;  // |y| and squares: zero is neutral for both
+    const float2 v = lane < warps ? red[lane] : make_float2(0.0f, 0.0f);  // squares and |h * w|: zero is neutral for both
+    sum = v.x, top = v.y;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = MAX ? max_nan(v, w) : v + w;
-    }
-    return v;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
 }
 
 // Columns c .. c + 7 of row `row` of h; columns past the row's end are zero.  ALIGN 0: element by element.
@@ -122,24 +136,22 @@ __device__ __forceinline__ void store_sum(const NormArgs &a, long long row, int 
 }
 
 template <int ALIGN>
-__device__ __forceinline__ void store_q(const NormArgs &a, long long row, int c, const float (&y)[8], float inv) {
+__device__ __forceinline__ void store_q(const NormArgs &a, long long row, int c, const float (&y)[8], float inv, float factor) {
     uint8_t *p = a.q + row * a.cols + c;
-    uint32_t b[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = to_8bit(y[j], inv, a.format);
+    const uint2 b = to_8bit(y, inv, factor, a.format);
     if constexpr (ALIGN != 0) {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+        *reinterpret_cast<uint2 *>(p) = b;
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (c + j < a.cols) p[j] = (uint8_t)b[j];
+            if (c + j < a.cols) p[j] = (uint8_t)((j < 4 ? b.x : b.y) >> (8 * (j & 3)));
     }
 }
 
 __device__ __forceinline__ float largest(const float (&y)[8]) {
     float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(y[j]));
+    for (int j = 0; j < 8; j += 2) m = max3_nan(m, fabsf(y[j]), fabsf(y[j + 1]));
     return m;
 }
 // over the lanes of a group: 8 columns a lane, so 4, 8 or 16 neighbouring lanes
@@ -148,83 +160,138 @@ __device__ __forceinline__ float group_max(float m, int group) {
     return m;
 }
 
-// NV pieces of eight columns a thread stay in registers: blockDim.x * 8 * NV >= cols.
-template <class T, int ALIGN, int NV>
-__global__ void __launch_bounds__(1024) rmsnorm_kernel(NormArgs a) {
-    __shared__ float red[2][33];
+__device__ __forceinline__ void norm_copy16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void norm_copy8(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// NV pieces of eight columns a thread stay in registers: blockDim.x * 8 * NV >= cols.  STAGES > 0: the block's next rows are
+// under way to shared memory while it works on this one (a thread copies what it will read itself, so no barrier orders
+// them): a row's chain of loads, two reductions and stores would leave the memory idle otherwise.
+template <class T, int ALIGN, int NV, int STAGES>
+__global__ void __launch_bounds__(NV == 1 ? 1024 : 512) rmsnorm_kernel(NormArgs a) {
+    constexpr int UNITS = sizeof(T) / 2;  // 16-byte pieces of eight columns
+    extern __shared__ __align__(16) uint4 norm_stage[];  // [stage][x, residual][piece][unit][thread]
+    __shared__ float2 red[2][32];  // in turn for odd and even rows
     float w[8] = {};
     if (NV == 1 && threadIdx.x * 8 < a.cols) load_weight<ALIGN>(a, threadIdx.x * 8, w);
+    auto slot = [&](int stage, int array, int i, int u) { return norm_stage + (((stage * 2 + array) * NV + i) * UNITS + u) * blockDim.x + threadIdx.x; };
+    auto prefetch = [&](long long row, int stage) {
+        if (row < a.rows) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * blockDim.x + threadIdx.x) * 8;
+                if (c >= a.cols) continue;
+#pragma unroll
+                for (int array = 0; array < 2; ++array) {
+                    if (array == 1 && !a.residual) continue;
+                    const T *p = array == 0 ? static_cast<const T *>(a.x) + row * a.x_stride + c : static_cast<const T *>(a.residual) + row * a.cols + c;
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u) {
+                        const char *src = reinterpret_cast<const char *>(p) + 16 * u;
+                        char *dst = reinterpret_cast<char *>(slot(stage, array, i, u));
+                        if constexpr (ALIGN == 16) norm_copy16(dst, src);
+                        else norm_copy8(dst, src), norm_copy8(dst + 8, src + 8);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if constexpr (STAGES > 0)
+        for (int k = 0; k < STAGES - 1; ++k) prefetch(blockIdx.x + (long long)k * gridDim.x, k);
+    int stage = 0, turn = 0;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float h[NV][8], sum = 0.0f;
+        if constexpr (STAGES > 0) {
+            prefetch(row + (long long)(STAGES - 1) * gridDim.x, stage == 0 ? STAGES - 1 : stage - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * blockDim.x + threadIdx.x) * 8;
-            if (c < a.cols) {
-                load_sum<T, ALIGN>(a, row, c, h[i]);
-            } else {
+            if (c >= a.cols) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] = 0.0f;
+                continue;
+            }
+            if constexpr (STAGES > 0) {
+                uint4 raw[UNITS];
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) raw[u] = *slot(stage, 0, i, u);
+                load8<16>(reinterpret_cast<const T *>(raw), h[i]);
+                if (a.residual) {
+                    float f[8];
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u) raw[u] = *slot(stage, 1, i, u);
+                    load8<16>(reinterpret_cast<const T *>(raw), f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[i][j] += f[j];
+                }
+            } else {
+                load_sum<T, ALIGN>(a, row, c, h[i]);
             }
         }
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        float top = 0.0f, part[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
-            if (c < a.cols) store_sum<T, ALIGN>(a, row, c, h[i]);
-        }
-        const float rstd = rsqrtf(__fdiv_rn(block_reduce<false>(sum, red[0]), (float)a.cols) + a.eps);
-        float top = 0.0f;
+            if (c < a.cols) {
+                store_sum<T, ALIGN>(a, row, c, h[i]);
+                if (NV > 1) load_weight<ALIGN>(a, c, w);
+            }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * blockDim.x + threadIdx.x) * 8;
-            if (NV > 1 && c < a.cols) load_weight<ALIGN>(a, c, w);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * rstd * w[j];
-            if (a.group == 0) top = max_nan(top, largest(h[i]));
+            for (int j = 0; j < 8; ++j) h[i][j] *= w[j];
+            part[i] = largest(h[i]);
+            top = max_nan(top, part[i]);
         }
+        turn ^= 1;
+        block_reduce(sum, top, red[turn]);
+        const float rstd = rsqrtf(sum * a.inv_cols + a.eps);
         float inv;
         if (a.group == 0) {
-            const float scale = group_scale(block_reduce<true>(top, red[1]), a.format, inv);
+            const float scale = group_scale(top * rstd, a.format, inv);
             if (threadIdx.x == 0) a.scales[row] = scale;
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * blockDim.x + threadIdx.x) * 8;
             if (a.group != 0) {
-                const float scale = group_scale(group_max(largest(h[i]), a.group), a.format, inv);
-                if (c < a.cols && c % a.group == 0) a.scales[row * a.groups + c / a.group] = scale;
+                const float scale = group_scale(group_max(part[i], a.group) * rstd, a.format, inv);
+                if (c < a.cols && (c & (a.group - 1)) == 0) a.scales[row * a.groups + (c >> a.group_shift)] = scale;
             }
-            if (c < a.cols) store_q<ALIGN>(a, row, c, h[i], inv);
+            if (c < a.cols) store_q<ALIGN>(a, row, c, h[i], inv, inv * rstd);
         }
     }
 }
 
-// Rows that outgrow the registers: the row is read once for its sum of squares, once more for a scale a row, and once
-// for its values; residual_out is written in that last pass, so that it may be the residual (or x) itself.
+// Rows that outgrow the registers: the row is read once for its sum of squares and its largest value, and once for its
+// values; residual_out is written in that second pass, so that it may be the residual (or x) itself.
 template <class T, int ALIGN>
 __global__ void __launch_bounds__(1024) rmsnorm_long_kernel(NormArgs a) {
-    __shared__ float red[2][33];
+    __shared__ float2 red[2][32];
+    int turn = 0;
     const int step = blockDim.x * 8, spans = (a.cols + step - 1) / step;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float sum = 0.0f, top = 0.0f, inv = 0.0f;
         for (int c = threadIdx.x * 8; c < a.cols; c += step) {
-            float h[8];
+            float h[8], w[8];
             load_sum<T, ALIGN>(a, row, c, h);
+            load_weight<ALIGN>(a, c, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(h[j], h[j], sum);
+            for (int j = 0; j < 8; ++j) sum = fmaf(h[j], h[j], sum), h[j] *= w[j];
+            top = max_nan(top, largest(h));
         }
-        const float rstd = rsqrtf(__fdiv_rn(block_reduce<false>(sum, red[0]), (float)a.cols) + a.eps);
+        turn ^= 1;
+        block_reduce(sum, top, red[turn]);
+        const float rstd = rsqrtf(sum * a.inv_cols + a.eps);
         if (a.group == 0) {
-            for (int c = threadIdx.x * 8; c < a.cols; c += step) {
-                float h[8], w[8];
-                load_sum<T, ALIGN>(a, row, c, h);
-                load_weight<ALIGN>(a, c, w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) h[j] = h[j] * rstd * w[j];
-                top = max_nan(top, largest(h));
-            }
-            const float scale = group_scale(block_reduce<true>(top, red[1]), a.format, inv);
+            const float scale = group_scale(top * rstd, a.format, inv);
             if (threadIdx.x == 0) a.scales[row] = scale;
         }
         for (int s = 0; s < spans; ++s) {  // whole warps take part in the groups' shuffles
@@ -236,24 +303,25 @@ __global__ void __launch_bounds__(1024) rmsnorm_long_kernel(NormArgs a) {
                 store_sum<T, ALIGN>(a, row, c, h);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = h[j] * rstd * w[j];
+            for (int j = 0; j < 8; ++j) h[j] *= w[j];
             if (a.group != 0) {
-                const float scale = group_scale(group_max(largest(h), a.group), a.format, inv);
-                if (c < a.cols && c % a.group == 0) a.scales[row * a.groups + c / a.group] = scale;
+                const float scale = group_scale(group_max(largest(h), a.group) * rstd, a.format, inv);
+                if (c < a.cols && (c & (a.group - 1)) == 0) a.scales[row * a.groups + (c >> a.group_shift)] = scale;
             }
-            if (c < a.cols) store_q<ALIGN>(a, row, c, h, inv);
+            if (c < a.cols) store_q<ALIGN>(a, row, c, h, inv, inv * rstd);
         }
     }
 }
 
-template <class T, int ALIGN, int NV>
+template <class T, int ALIGN, int NV, int STAGES>
 static int launch_norm(const NormArgs &a, int threads, const DeviceInfo *di, cudaStream_t s) {
+    const size_t smem = (size_t)STAGES * 2 * NV * sizeof(T) * 8 * threads;
     int st;
     if constexpr (NV > 0) {
-        st = ensure_kernel<rmsnorm_kernel<T, ALIGN, NV>, 0>(di);
+        st = ensure_kernel<rmsnorm_kernel<T, ALIGN, NV, STAGES>, STAGES ? KERNEL_OPTIN_SMEM | KERNEL_MAX_CARVEOUT : 0>(di);
         if (st) return st;
-        const int grid = (int)min((long long)a.rows, (long long)di->sm_count * (2048 / threads));
-        rmsnorm_kernel<T, ALIGN, NV><<<grid, threads, 0, s>>>(a);
+        const int grid = (int)min((long long)a.rows, STAGES ? max(1LL, (long long)di->sm_count * (long long)(200 * 1024 / (smem + 1024))) : (long long)di->sm_count * (2048 / threads));
+        rmsnorm_kernel<T, ALIGN, NV, STAGES><<<grid, threads, smem, s>>>(a);
     } else {
         st = ensure_kernel<rmsnorm_long_kernel<T, ALIGN>, 0>(di);
         if (st) return st;
@@ -266,11 +334,14 @@ static int launch_norm(const NormArgs &a, int threads, const DeviceInfo *di, cud
 template <class T, int ALIGN>
 static int dispatch_norm(const NormArgs &a, const DeviceInfo *di, cudaStream_t s) {
     const int pieces = (a.cols + 7) / 8;
-    const int threads = pieces >= 1024 ? 1024 : (pieces + 31) / 32 * 32;
-    if (pieces <= 1024) return launch_norm<T, ALIGN, 1>(a, threads, di, s);
-    if (pieces <= 2048) return launch_norm<T, ALIGN, 2>(a, (pieces + 63) / 64 * 32, di, s);
-    if (pieces <= 4096) return launch_norm<T, ALIGN, 4>(a, (pieces + 127) / 128 * 32, di, s);
-    return launch_norm<T, ALIGN, 0>(a, 1024, di, s);
+    if (pieces <= 1024 && a.rows < 2 * di->sm_count) return launch_norm<T, ALIGN, 1, 0>(a, (pieces + 31) / 32 * 32, di, s);
+    if constexpr (ALIGN != 0) {
+        // three stages of rows of up to 8192 16-bit columns leave room for two blocks an SM at least
+        if (pieces <= 1024 * 2 / (int)sizeof(T)) return launch_norm<T, ALIGN, 2, 3>(a, (pieces + 63) / 64 * 32, di, s);
+    }
+    if (pieces <= 2048) return launch_norm<T, ALIGN, 4, 0>(a, (pieces + 127) / 128 * 32, di, s);
+    if (pieces <= 4096) return launch_norm<T, ALIGN, 8, 0>(a, (pieces + 255) / 256 * 32, di, s);
+    return launch_norm<T, ALIGN, 0, 0>(a, 1024, di, s);
 }
 
 template <class T>
@@ -302,7 +373,7 @@ extern "C" int tb200_rmsnorm_quant(int rows, int cols, int type, const void *x, 
     int st;
     const DeviceInfo *di = device_info(&st);
     if (!di) return st;
-    NormArgs a{x, residual, residual_out, weight, q, scales, x_stride, eps, rows, cols, group, group ? (cols + group - 1) / group : 1, format};
+    NormArgs a{x, residual, residual_out, weight, q, scales, x_stride, eps, 1.0f / (float)cols, rows, cols, group, group ? __builtin_ctz(group) : 0, group ? (cols + group - 1) / group : 1, format};
     cudaStream_t s = (cudaStream_t)stream;
     if (type == TB200_TYPE_F32) return dispatch_norm_align<float>(a, di, s);
     if (type == TB200_TYPE_F16) return dispatch_norm_align<__half>(a, di, s);
