@@ -24,28 +24,30 @@ struct PlanArgs {
     int requests, page_size, max_pages, max_tokens, num_free;
 };
 
-// Exclusive prefix of one value a thread over the block, and the total.  `warp_sums`: 33 words, free after the call's
-// first barrier of the next use.
-__device__ __forceinline__ long long block_scan(long long v, long long *warp_sums, long long &total) {
+// Exclusive prefix sums of one value a thread over the block, and the total, both held at `most` (a sum held at a limit is
+// associative, and 32 bits take lengths whose true sum they could not).  `warp_sums`: 32 words.
+__device__ __forceinline__ unsigned block_scan(unsigned v, unsigned most, unsigned *warp_sums, unsigned &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    long long inc = v;
+    unsigned inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long w = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += w;
+        const unsigned w = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc = min(inc + w, most);
     }
+    unsigned before = __shfl_up_sync(0xffffffffu, inc, 1);
+    if (lane == 0) before = 0;
     __syncthreads();
     if (lane == 31) warp_sums[warp] = inc;
     __syncthreads();
-    const long long ws = lane < warps ? warp_sums[lane] : 0;
-    long long winc = ws;
+    unsigned winc = lane < warps ? warp_sums[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long w = __shfl_up_sync(0xffffffffu, winc, o);
-        if (lane >= o) winc += w;
+        const unsigned w = __shfl_up_sync(0xffffffffu, winc, o);
+        if (lane >= o) winc = min(winc + w, most);
     }
     total = __shfl_sync(0xffffffffu, winc, 31);
-    return __shfl_sync(0xffffffffu, winc - ws, warp) + inc - v;
+    const unsigned others = __shfl_sync(0xffffffffu, winc, warp ? warp - 1 : 0);
+    return warp ? min(others + before, most) : before;
 }
 
 // the last r with first[r] <= at (first[0] = 0 <= at; requests without rows share their successor's first row)
@@ -59,43 +61,52 @@ __device__ __forceinline__ int find_request(const int *first, int requests, int 
     return lo;
 }
 
+// PER: requests a thread takes in the prefix sums (PER * blockDim.x >= requests), neighbours, in registers: their lengths
+// are read once, all at the same time.
+template <int PER>
 __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PlanArgs a) {
     extern __shared__ int plan_smem[];
-    __shared__ long long warp_sums[33];
+    __shared__ unsigned warp_sums[32];
     int *first_row = plan_smem;                     // [requests + 1]
     int *first_page = plan_smem + a.requests + 1;   // [requests + 1]: fresh pages
-    const int R = a.requests, P = a.page_size;
-    const int per = (R + blockDim.x - 1) / blockDim.x, r0 = min(R, (int)threadIdx.x * per), r1 = min(R, r0 + per);
-    const long long room = (long long)a.max_pages * P;
+    const int R = a.requests, P = a.page_size, r0 = threadIdx.x * PER;
+    const int room = a.max_pages * P;
+    const unsigned most = (unsigned)a.max_tokens;
 
-    long long rows = 0, asked = 0;
-    for (int r = r0; r < r1; ++r) {
-        const int c = max(0, a.cached_lens[r]), n = max(0, a.new_lens[r]);
-        asked += n;
-        rows += min((long long)n, max(0LL, room - c));
+    int c[PER], n[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        c[i] = r0 + i < R ? a.cached_lens[r0 + i] : 0;
+        n[i] = r0 + i < R ? a.new_lens[r0 + i] : 0;
     }
-    long long total_rows, total_asked = 0, total_pages;
-    long long at = block_scan(rows, warp_sums, total_rows);
-    if (blockIdx.x == 0) block_scan(asked, warp_sums, total_asked);  // only counts[] needs it
-    long long pages = 0;
-    for (int r = r0; r < r1; ++r) {
-        const int c = max(0, a.cached_lens[r]);
-        const long long n = min((long long)max(0, a.new_lens[r]), max(0LL, room - c));
-        const int b = (int)min(at, (long long)a.max_tokens), e = (int)min(at + n, (long long)a.max_tokens);
-        first_row[r] = b;
-        if (e > b) pages += (c + (e - b) + P - 1) / P - (c + P - 1) / P;
-        at += n;
+    unsigned rows = 0, asked = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        c[i] = max(0, c[i]), n[i] = max(0, n[i]);
+        asked = min(asked + (unsigned)n[i], 0x7FFFFFFFu);
+        n[i] = min(n[i], max(0, room - min(c[i], room)));
+        rows = min(rows + (unsigned)n[i], most);
     }
-    const int used = (int)min(total_rows, (long long)a.max_tokens);
-    if (threadIdx.x == 0) first_row[R] = used;
-    long long page = block_scan(pages, warp_sums, total_pages);
-    __syncthreads();
-    for (int r = r0; r < r1; ++r) {
-        const int c = max(0, a.cached_lens[r]), n = first_row[r + 1] - first_row[r];
-        first_page[r] = (int)page;
-        if (n > 0) page += (c + n + P - 1) / P - (c + P - 1) / P;
+    unsigned total_rows, total_asked = 0, total_pages;
+    unsigned at = block_scan(rows, most, warp_sums, total_rows);
+    if (blockIdx.x == 0) block_scan(asked, 0x7FFFFFFFu, warp_sums, total_asked);  // only counts[] needs it
+    unsigned pages = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int b = (int)at, e = (int)min(at + (unsigned)n[i], most);
+        if (r0 + i < R) first_row[r0 + i] = b;
+        at = (unsigned)e;
+        n[i] = e > b ? (c[i] + (e - b) + P - 1) / P - (c[i] + P - 1) / P : 0;  // from here on its fresh pages
+        pages += n[i];
     }
-    if (threadIdx.x == 0) first_page[R] = (int)total_pages;
+    const int used = (int)total_rows;
+    int page = (int)block_scan(pages, 0x7FFFFFFFu, warp_sums, total_pages);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (r0 + i < R) first_page[r0 + i] = page;
+        page += n[i];
+    }
+    if (threadIdx.x == 0) first_row[R] = used, first_page[R] = (int)total_pages;
     __syncthreads();
 
     if (blockIdx.x == 0) {
@@ -106,32 +117,66 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(PlanArgs a) {
         if (threadIdx.x == 0) {
             a.cu_new[R] = used;
             a.counts[0] = used;
-            a.counts[1] = (int)min(total_asked, 0x7FFFFFFFLL);
-            a.counts[2] = (int)min(total_pages, (long long)a.num_free);
+            a.counts[1] = (int)total_asked;
+            a.counts[2] = min((int)total_pages, a.num_free);
             a.counts[3] = (int)total_pages;
         }
     }
     const long long stride = (long long)gridDim.x * blockDim.x, me = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    for (long long t = me; t < a.max_tokens; t += stride) {
-        int position = -1;
-        long long slot = -1;
-        if (t < used) {
-            const int r = find_request(first_row, R, (int)t), c = max(0, a.cached_lens[r]);
-            position = c + (int)t - first_row[r];
-            const int index = position / P, held = (c + P - 1) / P;
-            // entries below `held` are not written by this launch; the others come from the free list directly
-            const int f = first_page[r] + index - held;
-            const int entry = index < held ? a.block_table[(long long)r * a.max_pages + index] : f < a.num_free ? a.free_pages[f] : -1;
-            if (entry >= 0) slot = (long long)entry * P + (position - index * P);
+    const bool wide = (((uintptr_t)a.positions | (uintptr_t)a.slots) & 15) == 0;
+    // four rows in a line a thread: one search, one division and one table entry serve what they share
+    for (long long t0 = 4 * me; t0 < a.max_tokens; t0 += 4 * stride) {
+        int r = 0, position = 0, off = 0, end = -1, p[4];
+        long long page_slot = -1, slot[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long t = t0 + i;
+            p[i] = -1, slot[i] = -1;
+            if (t >= used) continue;
+            const bool next = t >= end;
+            if (next) {
+                if (end < 0) r = find_request(first_row, R, (int)t);
+                else do ++r;
+                    while (first_row[r + 1] <= t);
+                end = first_row[r + 1];
+                position = max(0, a.cached_lens[r]) + (int)t - first_row[r];
+                off = position % P;
+            }
+            if (next || off == P) {
+                if (!next) off = 0;
+                // entries below `held` are not written by this launch; the others come from the free list directly
+                const int index = position / P, held = (max(0, a.cached_lens[r]) + P - 1) / P, f = first_page[r] + index - held;
+                const int entry = index < held ? a.block_table[(long long)r * a.max_pages + index] : f < a.num_free ? a.free_pages[f] : -1;
+                page_slot = entry >= 0 ? (long long)entry * P : -1;
+            }
+            p[i] = position++;
+            if (page_slot >= 0) slot[i] = page_slot + off;
+            ++off;
         }
-        a.positions[t] = position;
-        a.slots[t] = slot;
+        if (wide && t0 + 4 <= a.max_tokens) {
+            *reinterpret_cast<int4 *>(a.positions + t0) = make_int4(p[0], p[1], p[2], p[3]);
+            *reinterpret_cast<longlong2 *>(a.slots + t0) = make_longlong2(slot[0], slot[1]);
+            *reinterpret_cast<longlong2 *>(a.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t0 + i < a.max_tokens) a.positions[t0 + i] = p[i], a.slots[t0 + i] = slot[i];
+        }
     }
-    for (long long f = me; f < total_pages; f += stride) {
+    for (long long f = me; f < (long long)total_pages; f += stride) {
         const int r = find_request(first_page, R, (int)f);
         const int index = (max(0, a.cached_lens[r]) + P - 1) / P + (int)f - first_page[r];
         a.block_table[(long long)r * a.max_pages + index] = f < a.num_free ? a.free_pages[f] : -1;
     }
+}
+
+template <int PER>
+static int launch_plan(const PlanArgs &a, int threads, const DeviceInfo *di, cudaStream_t s) {
+    const int st = ensure_kernel<paged_plan_kernel<PER>>(di);
+    if (st) return st;
+    const int grid = max(1, min((a.max_tokens + 4 * threads - 1) / (4 * threads), di->sm_count));
+    paged_plan_kernel<PER><<<grid, threads, 2 * (size_t)(a.requests + 1) * sizeof(int), s>>>(a);
+    return check_launch();
 }
 
 // ---------------------------------------------------------------------------
@@ -312,13 +357,12 @@ extern "C" int tb200_paged_plan(int requests, int page_size, int max_pages, int 
     int st;
     const DeviceInfo *di = device_info(&st);
     if (!di) return st;
-    st = ensure_kernel<paged_plan_kernel>(di);
-    if (st) return st;
     PlanArgs a{cached_lens, new_lens, free_pages, block_table, cu_new, kv_lens, positions, counts, slots, requests, page_size, max_pages, max_tokens, num_free};
-    const int threads = requests <= 256 && max_tokens <= 256 ? 256 : PLAN_THREADS;
-    const int grid = max(1, min((max_tokens + threads - 1) / threads, di->sm_count));
-    paged_plan_kernel<<<grid, threads, 2 * (size_t)(requests + 1) * sizeof(int), (cudaStream_t)stream>>>(a);
-    return check_launch();
+    cudaStream_t s = (cudaStream_t)stream;
+    if (requests <= 256 && max_tokens <= 1024) return launch_plan<1>(a, 256, di, s);
+    if (requests <= PLAN_THREADS) return launch_plan<1>(a, PLAN_THREADS, di, s);
+    if (requests <= 4 * PLAN_THREADS) return launch_plan<4>(a, PLAN_THREADS, di, s);
+    return launch_plan<16>(a, PLAN_THREADS, di, s);
 }
 
 extern "C" int tb200_rope_append(int tokens, int q_heads, int kv_heads, int head_dim, int in_type, const void *q, const void *k, const void *v,

@@ -171,7 +171,7 @@ __device__ __forceinline__ void norm_copy8(void *dst, const void *src) {
 // under way to shared memory while it works on this one (a thread copies what it will read itself, so no barrier orders
 // them): a row's chain of loads, two reductions and stores would leave the memory idle otherwise.
 template <class T, int ALIGN, int NV, int STAGES>
-__global__ void __launch_bounds__(NV == 1 ? 1024 : 512) rmsnorm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(NV <= 2 && STAGES == 0 ? 1024 : 512) rmsnorm_kernel(NormArgs a) {
     constexpr int UNITS = sizeof(T) / 2;  // 16-byte pieces of eight columns
     extern __shared__ __align__(16) uint4 norm_stage[];  // [stage][x, residual][piece][unit][thread]
     __shared__ float2 red[2][32];  // in turn for odd and even rows
@@ -339,7 +339,7 @@ static int dispatch_norm(const NormArgs &a, const DeviceInfo *di, cudaStream_t s
         // three stages of rows of up to 8192 16-bit columns leave room for two blocks an SM at least
         if (pieces <= 1024 * 2 / (int)sizeof(T)) return launch_norm<T, ALIGN, 2, 3>(a, (pieces + 63) / 64 * 32, di, s);
     }
-    if (pieces <= 2048) return launch_norm<T, ALIGN, 4, 0>(a, (pieces + 127) / 128 * 32, di, s);
+    if (pieces <= 2048) return launch_norm<T, ALIGN, 2, 0>(a, (pieces + 63) / 64 * 32, di, s);
     if (pieces <= 4096) return launch_norm<T, ALIGN, 8, 0>(a, (pieces + 255) / 256 * 32, di, s);
     return launch_norm<T, ALIGN, 0, 0>(a, 1024, di, s);
 }
