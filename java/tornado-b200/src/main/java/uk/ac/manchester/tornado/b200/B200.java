@@ -10,6 +10,9 @@ import uk.ac.manchester.tornado.api.types.arrays.ByteArray;
 import uk.ac.manchester.tornado.api.types.arrays.FloatArray;
 import uk.ac.manchester.tornado.api.types.arrays.HalfFloatArray;
 import uk.ac.manchester.tornado.api.types.arrays.Int8Array;
+import uk.ac.manchester.tornado.api.types.arrays.IntArray;
+import uk.ac.manchester.tornado.api.types.arrays.LongArray;
+import uk.ac.manchester.tornado.api.types.arrays.TornadoNativeArray;
 
 /**
  * Factories of the {@code b200/linalg} library tasks: dense and quantised matrix-vector and
@@ -200,5 +203,106 @@ public final class B200 {
         check(m >= 0 && n >= 0 && k >= 0, "B200 hgemmF32 requires non-negative sizes; got m=" + m + ", n=" + n + ", k=" + k);
         check(a.getSize() >= (long) m * k && b.getSize() >= (long) k * n && c.getSize() >= (long) m * n, "B200 hgemmF32: array too small");
         return descriptor("hgemmF32", new Object[] { m, n, k, a, b, c }, 5, false, null);
+    }
+
+    // ---- decoder layer: what lies between its quantised products ----
+
+    public static final int TYPE_F32 = 0, TYPE_F16 = 1, TYPE_BF16 = 2;
+    public static final int QUANT_INT8 = 0, QUANT_E4M3 = 1, QUANT_E5M2 = 2;
+
+    private static int elementType(String name, TornadoNativeArray array) {
+        if (array instanceof FloatArray) {
+            return TYPE_F32;
+        }
+        if (array instanceof HalfFloatArray) {
+            return TYPE_F16;
+        }
+        check(array instanceof BFloat16Array, "B200 " + name + " does not take a " + array.getClass().getSimpleName());
+        return TYPE_BF16;
+    }
+
+    private static LibraryTaskDescriptor descriptor(String function, Object[] params, int[] readWrite, int[] writeOnly) {
+        Access[] access = new Access[params.length];
+        Arrays.fill(access, Access.READ_ONLY);
+        for (int i : readWrite) {
+            access[i] = Access.READ_WRITE;
+        }
+        for (int i : writeOnly) {
+            access[i] = Access.WRITE_ONLY;
+        }
+        return new LibraryTaskDescriptor().withLibrary(LIBRARY_NAME).withFunction(function).withParameters(params).withAccess(access);
+    }
+
+    private static void checkNorm(String name, int rows, int cols, TornadoNativeArray x, FloatArray weight, float eps, int format, int group, TornadoNativeArray q, FloatArray scales) {
+        check(rows >= 0 && cols >= 1, "B200 " + name + " requires rows >= 0 and cols >= 1; got rows=" + rows + ", cols=" + cols);
+        check(format >= QUANT_INT8 && format <= QUANT_E5M2, "B200 " + name + " knows the formats 0 (int8), 1 (e4m3), 2 (e5m2); got " + format);
+        check(group == 0 || group == 32 || group == 64 || group == 128, "B200 " + name + " requires groups of 32, 64 or 128 columns, or 0 for a scale per row; got " + group);
+        check(eps >= 0.0f && eps <= Float.MAX_VALUE, "B200 " + name + " requires a finite eps >= 0; got " + eps);
+        long groups = group == 0 ? 1 : (cols + group - 1) / group;
+        check(x.getSize() >= (long) rows * cols && weight.getSize() >= cols && q.getSize() >= (long) rows * cols && scales.getSize() >= rows * groups, "B200 " + name + ": array too small");
+    }
+
+    /** RMS norm of x's rows as 8-bit values (an Int8Array or ByteArray) with a scale per group of columns (0: per row). */
+    public static LibraryTaskDescriptor rmsnormQuant(int rows, int cols, TornadoNativeArray x, FloatArray weight, float eps, int format, int group, TornadoNativeArray q, FloatArray scales) {
+        checkNorm("rmsnormQuant", rows, cols, x, weight, eps, format, group, q, scales);
+        return descriptor("rmsnormQuant", new Object[] { rows, cols, elementType("rmsnormQuant", x), x, weight, eps, format, group, q, scales }, new int[] {}, new int[] { 8, 9 });
+    }
+
+    /** rmsnormQuant of {@code residual + x}; the sum, rounded to the arrays' type, replaces {@code residual}. */
+    public static LibraryTaskDescriptor addRmsnormQuant(int rows, int cols, TornadoNativeArray x, TornadoNativeArray residual, FloatArray weight, float eps, int format, int group,
+            TornadoNativeArray q, FloatArray scales) {
+        checkNorm("addRmsnormQuant", rows, cols, x, weight, eps, format, group, q, scales);
+        check(residual.getClass() == x.getClass() && residual.getSize() >= (long) rows * cols, "B200 addRmsnormQuant: residual differs from x in type, or is too small");
+        return descriptor("addRmsnormQuant", new Object[] { rows, cols, elementType("addRmsnormQuant", x), x, residual, weight, eps, format, group, q, scales }, new int[] { 4 }, new int[] { 9, 10 });
+    }
+
+    /** Lays out a step of a paged cache: fresh pages from freePages into the table rows, each token row's position and slot. */
+    public static LibraryTaskDescriptor pagedPlan(int requests, int pageSize, int maxPages, int maxTokens, IntArray cachedLens, IntArray newLens, IntArray freePages, IntArray blockTable,
+            IntArray cuNew, IntArray kvLens, IntArray positions, LongArray slots, IntArray counts) {
+        check(requests >= 0 && requests <= 16384, "B200 pagedPlan requires 0 <= requests <= 16384; got " + requests);
+        check(pageSize >= 1 && maxPages >= 0 && (long) maxPages * pageSize <= 1L << 30, "B200 pagedPlan requires pages of at least one position and at most 2^30 positions in a table row");
+        check(maxTokens >= 0 && maxTokens <= 1 << 30, "B200 pagedPlan requires 0 <= maxTokens <= 2^30; got " + maxTokens);
+        check(cachedLens.getSize() >= requests && newLens.getSize() >= requests && blockTable.getSize() >= (long) requests * maxPages && cuNew.getSize() >= requests + 1
+                && kvLens.getSize() >= requests && positions.getSize() >= maxTokens && slots.getSize() >= maxTokens && counts.getSize() >= 4, "B200 pagedPlan: array too small");
+        return descriptor("pagedPlan", new Object[] { requests, pageSize, maxPages, maxTokens, freePages.getSize(), cachedLens, newLens, freePages, blockTable, cuNew, kvLens, positions, slots,
+                counts }, new int[] { 8 }, new int[] { 9, 10, 11, 12, 13 });
+    }
+
+    private static int cachePages(String name, int kvHeads, int headDim, int pageSize, TornadoNativeArray kCache, TornadoNativeArray vCache) {
+        check(kvHeads >= 1 && headDim >= 1 && pageSize >= 1, "B200 " + name + " requires kvHeads, headDim and pageSize >= 1");
+        long per = (long) kvHeads * headDim * pageSize;
+        check(kCache.getClass() == vCache.getClass() && !(kCache instanceof FloatArray), "B200 " + name + " requires caches of one 16-bit type");
+        check(kCache.getSize() == vCache.getSize() && kCache.getSize() % per == 0, "B200 " + name + ": the caches are not both whole pages of kvHeads x pageSize x headDim elements");
+        return (int) (kCache.getSize() / per);
+    }
+
+    /** Rotates queries and keys of projection rows [tokens][(qHeads + 2 kvHeads) headDim], stores queries in q, keys and values at their slots. */
+    public static LibraryTaskDescriptor ropeAppend(int tokens, int qHeads, int kvHeads, int headDim, TornadoNativeArray qkv, FloatArray cosTable, FloatArray sinTable, int rotDim,
+            boolean interleaved, IntArray positions, LongArray slots, int pageSize, TornadoNativeArray q, TornadoNativeArray kCache, TornadoNativeArray vCache) {
+        int pages = cachePages("ropeAppend", kvHeads, headDim, pageSize, kCache, vCache);
+        check(tokens >= 0 && qHeads >= 0 && rotDim >= 0 && rotDim <= headDim && rotDim % 2 == 0, "B200 ropeAppend requires tokens, qHeads >= 0 and an even rotDim of at most headDim");
+        int tableRows = rotDim == 0 ? 0 : (int) (Math.min(cosTable.getSize(), sinTable.getSize()) / (rotDim / 2));
+        check(qkv.getSize() >= (long) tokens * (qHeads + 2 * kvHeads) * headDim && q.getSize() >= (long) tokens * qHeads * headDim && positions.getSize() >= tokens && slots.getSize() >= tokens,
+                "B200 ropeAppend: array too small");
+        check(q.getClass() == kCache.getClass(), "B200 ropeAppend: q and the caches differ in type");
+        return descriptor("ropeAppend", new Object[] { tokens, qHeads, kvHeads, headDim, elementType("ropeAppend", qkv), qkv, cosTable, sinTable, tableRows, rotDim, interleaved ? 1 : 0,
+                positions, elementType("ropeAppend", kCache), q, pageSize, pages, slots, kCache, vCache }, new int[] { 13, 17, 18 }, new int[] {});
+    }
+
+    /** Causal attention of each request's new tokens over its pages of the cache, the new tokens included; window 0: no limit. */
+    public static LibraryTaskDescriptor pagedAttention(int tokens, int requests, int maxNew, int qHeads, int kvHeads, int headDim, TornadoNativeArray q, IntArray cuNew, IntArray kvLens,
+            IntArray blockTable, int pageSize, TornadoNativeArray kCache, TornadoNativeArray vCache, float scale, int window, TornadoNativeArray out) {
+        int pages = cachePages("pagedAttention", kvHeads, headDim, pageSize, kCache, vCache);
+        check(tokens >= 0 && requests >= 1 && maxNew >= 0 && window >= 0, "B200 pagedAttention requires tokens, maxNew, window >= 0 and requests >= 1");
+        check(qHeads >= kvHeads && qHeads % kvHeads == 0, "B200 pagedAttention requires qHeads to be a multiple of kvHeads; got " + qHeads + ", " + kvHeads);
+        check(headDim % 8 == 0 && headDim <= 256, "B200 pagedAttention requires headDim to be a multiple of 8 up to 256; got " + headDim);
+        check(scale > 0.0f && scale <= Float.MAX_VALUE, "B200 pagedAttention requires a finite scale > 0; got " + scale);
+        int maxPages = (int) (blockTable.getSize() / requests);
+        check(blockTable.getSize() % requests == 0 && (long) maxPages * pageSize <= 1L << 30, "B200 pagedAttention: the table is not [requests][maxPages], or a row holds over 2^30 positions");
+        check(q.getSize() >= (long) tokens * qHeads * headDim && out.getSize() >= (long) tokens * qHeads * headDim && cuNew.getSize() >= requests + 1 && kvLens.getSize() >= requests,
+                "B200 pagedAttention: array too small");
+        check(q.getClass() == kCache.getClass() && out.getClass() == kCache.getClass(), "B200 pagedAttention: q, out and the caches differ in type");
+        return descriptor("pagedAttention", new Object[] { tokens, requests, maxNew, qHeads, kvHeads, headDim, elementType("pagedAttention", q), q, cuNew, kvLens, blockTable, maxPages, pageSize,
+                pages, kCache, vCache, scale, window, out }, new int[] { 18 }, new int[] {});
     }
 }

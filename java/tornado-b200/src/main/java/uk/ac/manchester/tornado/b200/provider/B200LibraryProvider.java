@@ -82,6 +82,7 @@ public final class B200LibraryProvider implements TornadoLibraryProvider {
             case "sgemv" -> B200Native.PREPARE_GEMV_F32;
             case "sgemm" -> B200Native.PREPARE_GEMM_F32;
             case "q8Gemv", "q8GemvBytes", "q4GemvBytes", "q8GemvBytesGrouped", "q4GemvBytesGrouped", "q8GemvBytesPacked", "q4GemvBytesPacked" -> B200Native.PREPARE_GEMV_QUANT;
+            case "rmsnormQuant", "addRmsnormQuant", "pagedPlan", "ropeAppend", "pagedAttention" -> B200Native.PREPARE_LAYER;
             default -> B200Native.PREPARE_GEMM_F16;
         };
     }
@@ -97,6 +98,9 @@ public final class B200LibraryProvider implements TornadoLibraryProvider {
         Object[] p = descriptor.getParameters();
         if (isQuantised(function) && descriptor.getTuning() instanceof B200Options options && options.exactInt) {
             ((B200Context) context).growWorkspace(B200Native.qxWorkspaceBytes((int) p[1], (int) p[2]));
+        }
+        if (function.equals("pagedAttention")) { // (tokens, requests, maxNew, qHeads, kvHeads, headDim, ...)
+            ((B200Context) context).growWorkspace(B200Native.pagedAttentionWorkspaceBytes((int) p[0], (int) p[1], (int) p[3], (int) p[4], (int) p[5]));
         }
         if (function.endsWith("Grouped") || function.endsWith("Packed")) { // (count, rows, cols, batch, ...): integer mode whatever the tuning
             ((B200Context) context).growWorkspace(B200Native.qxWorkspaceBytes((int) p[2], (int) p[3]));
@@ -195,6 +199,39 @@ public final class B200LibraryProvider implements TornadoLibraryProvider {
             case "gemmBiasRelu", "gemmBiasGelu", "gemmBiasSilu", "gemmBiasSigmoid", "gemmBiasTanh", "gemmBiasHardSwish" -> //
                     B200Native.gemmEx((int) inv.getArg(0), (int) inv.getArg(1), (int) inv.getArg(2), 0, inv.getDevicePointer(3), inv.getDevicePointer(4), //
                             1, inv.getDevicePointer(6), 1.0f, 0.0f, 0L, inv.getDevicePointer(5), fusedActivation(functionName), 1, ctx.stream);
+            // (rows, cols, type, x, weight, eps, format, group, q, scales)
+            case "rmsnormQuant" -> B200Native.rmsnormQuant((int) inv.getArg(0), (int) inv.getArg(1), (int) inv.getArg(2), inv.getDevicePointer(3), (long) (int) inv.getArg(1), 0L, 0L, //
+                    inv.getDevicePointer(4), (float) inv.getArg(5), (int) inv.getArg(6), (int) inv.getArg(7), inv.getDevicePointer(8), inv.getDevicePointer(9), ctx.stream);
+            // (rows, cols, type, x, residual, weight, eps, format, group, q, scales): the residual is updated in place
+            case "addRmsnormQuant" -> B200Native.rmsnormQuant((int) inv.getArg(0), (int) inv.getArg(1), (int) inv.getArg(2), inv.getDevicePointer(3), (long) (int) inv.getArg(1), //
+                    inv.getDevicePointer(4), inv.getDevicePointer(4), inv.getDevicePointer(5), (float) inv.getArg(6), (int) inv.getArg(7), (int) inv.getArg(8), inv.getDevicePointer(9), //
+                    inv.getDevicePointer(10), ctx.stream);
+            // (requests, pageSize, maxPages, maxTokens, numFree, cached, new, free, table, cu, kv, positions, slots, counts)
+            case "pagedPlan" -> B200Native.pagedPlan((int) inv.getArg(0), (int) inv.getArg(1), (int) inv.getArg(2), (int) inv.getArg(3), (int) inv.getArg(4), inv.getDevicePointer(5), //
+                    inv.getDevicePointer(6), inv.getDevicePointer(7), inv.getDevicePointer(8), inv.getDevicePointer(9), inv.getDevicePointer(10), inv.getDevicePointer(11), //
+                    inv.getDevicePointer(12), inv.getDevicePointer(13), ctx.stream);
+            // (tokens, qHeads, kvHeads, headDim, inType, qkv, cos, sin, tableRows, rotDim, interleaved, positions, cacheType, q, pageSize, numPages, slots, k, v)
+            case "ropeAppend" -> {
+                int qHeads = (int) inv.getArg(1);
+                int kvHeads = (int) inv.getArg(2);
+                int headDim = (int) inv.getArg(3);
+                long size = (int) inv.getArg(4) == B200.TYPE_F32 ? 4 : 2;
+                long row = (qHeads + 2L * kvHeads) * headDim;
+                long q = inv.getDevicePointer(5);
+                long k = q + (long) qHeads * headDim * size;
+                long v = k + (long) kvHeads * headDim * size;
+                yield B200Native.ropeAppend((int) inv.getArg(0), qHeads, kvHeads, headDim, (int) inv.getArg(4), q, k, v, row, row, row, inv.getDevicePointer(6), inv.getDevicePointer(7), //
+                        (int) inv.getArg(8), (int) inv.getArg(9), (int) inv.getArg(10), inv.getDevicePointer(11), (int) inv.getArg(12), inv.getDevicePointer(13), (int) inv.getArg(14), //
+                        (int) inv.getArg(15), inv.getDevicePointer(16), inv.getDevicePointer(17), inv.getDevicePointer(18), ctx.stream);
+            }
+            // (tokens, requests, maxNew, qHeads, kvHeads, headDim, type, q, cu, kv, table, maxPages, pageSize, numPages, k, v, scale, window, out)
+            case "pagedAttention" -> {
+                long row = (long) (int) inv.getArg(3) * (int) inv.getArg(5);
+                yield B200Native.pagedAttention((int) inv.getArg(0), (int) inv.getArg(1), (int) inv.getArg(2), (int) inv.getArg(3), (int) inv.getArg(4), (int) inv.getArg(5), (int) inv.getArg(6), //
+                        inv.getDevicePointer(7), row, inv.getDevicePointer(8), inv.getDevicePointer(9), inv.getDevicePointer(10), (int) inv.getArg(11), (int) inv.getArg(12), //
+                        (int) inv.getArg(13), inv.getDevicePointer(14), inv.getDevicePointer(15), (float) inv.getArg(16), (int) inv.getArg(17), inv.getDevicePointer(18), row, //
+                        ctx.workspacePtr, ctx.workspaceBytes, ctx.stream);
+            }
             default -> throw new TornadoRuntimeException("[ERROR] B200 function not supported: " + functionName);
         };
     }

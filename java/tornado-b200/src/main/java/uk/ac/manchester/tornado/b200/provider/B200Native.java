@@ -27,6 +27,7 @@ public final class B200Native {
     public static final int PREPARE_GEMV_QUANT = 2;
     public static final int PREPARE_GEMM_F32 = 4;
     public static final int PREPARE_GEMM_F16 = 8;
+    public static final int PREPARE_LAYER = 32;
 
     private static final Linker LINKER = Linker.nativeLinker();
     private static SymbolLookup lib;
@@ -42,6 +43,11 @@ public final class B200Native {
     private static MethodHandle sgemm;
     private static MethodHandle hgemmF32;
     private static MethodHandle qxWorkspaceBytes;
+    private static MethodHandle rmsnormQuant;
+    private static MethodHandle pagedPlan;
+    private static MethodHandle ropeAppend;
+    private static MethodHandle pagedAttention;
+    private static MethodHandle pagedAttentionWorkspaceBytes;
     private static MethodHandle deviceMalloc;
     private static MethodHandle deviceFree;
     private static MethodHandle statusString;
@@ -83,6 +89,11 @@ public final class B200Native {
         q4bGemvI8Grouped = handle("tb200_q4b_gemv_i8_grouped", grouped);
         sgemm = handle("tb200_sgemm", FunctionDescriptor.of(JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_LONG, JAVA_LONG, JAVA_FLOAT, JAVA_LONG, JAVA_LONG));
         hgemmF32 = handle("tb200_hgemm_f32", FunctionDescriptor.of(JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG));
+        rmsnormQuant = handle("tb200_rmsnorm_quant", FunctionDescriptor.of(JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_FLOAT, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG));
+        pagedPlan = handle("tb200_paged_plan", FunctionDescriptor.of(JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG));
+        ropeAppend = handle("tb200_rope_append", FunctionDescriptor.of(JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_INT, JAVA_LONG, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG));
+        pagedAttention = handle("tb200_paged_attention", FunctionDescriptor.of(JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_FLOAT, JAVA_INT, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG, JAVA_LONG));
+        pagedAttentionWorkspaceBytes = handle("tb200_paged_attention_workspace_bytes", FunctionDescriptor.of(JAVA_LONG, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT));
         qxWorkspaceBytes = handle("tb200_qx_workspace_bytes", FunctionDescriptor.of(JAVA_LONG, JAVA_INT, JAVA_INT));
         deviceMalloc = handle("tb200_device_malloc", FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS));
         deviceFree = handle("tb200_device_free", FunctionDescriptor.of(JAVA_INT, JAVA_LONG));
@@ -247,6 +258,51 @@ public final class B200Native {
             int batchCount, long stream) {
         try {
             return (int) gemmEx.invokeExact(m, n, k, inType, a, b, outType, d, alpha, beta, c, bias, activation, batchCount, stream);
+        } catch (Throwable t) {
+            throw wrap(t);
+        }
+    }
+
+    /** RMS norm with an 8-bit output; residual and residualOut may be 0. */
+    public static int rmsnormQuant(int rows, int cols, int type, long x, long xStride, long residual, long residualOut, long weight, float eps, int format, int group, long q, long scales, long stream) {
+        try {
+            return (int) rmsnormQuant.invokeExact(rows, cols, type, x, xStride, residual, residualOut, weight, eps, format, group, q, scales, stream);
+        } catch (Throwable t) {
+            throw wrap(t);
+        }
+    }
+
+    /** Block table entries, positions and slots of a step. */
+    public static int pagedPlan(int requests, int pageSize, int maxPages, int maxTokens, int numFree, long cachedLens, long newLens, long freePages, long blockTable, long cuNew, long kvLens, long positions, long slots, long counts, long stream) {
+        try {
+            return (int) pagedPlan.invokeExact(requests, pageSize, maxPages, maxTokens, numFree, cachedLens, newLens, freePages, blockTable, cuNew, kvLens, positions, slots, counts, stream);
+        } catch (Throwable t) {
+            throw wrap(t);
+        }
+    }
+
+    /** Rotary positions and the write into the paged cache. */
+    public static int ropeAppend(int tokens, int qHeads, int kvHeads, int headDim, int inType, long q, long k, long v, long qStride, long kStride, long vStride, long cosTable, long sinTable, int tableRows, int rotDim, int interleaved, long positions, int cacheType, long qOut, int pageSize, int numPages, long slots, long kCache, long vCache, long stream) {
+        try {
+            return (int) ropeAppend.invokeExact(tokens, qHeads, kvHeads, headDim, inType, q, k, v, qStride, kStride, vStride, cosTable, sinTable, tableRows, rotDim, interleaved, positions, cacheType, qOut, pageSize, numPages, slots, kCache, vCache, stream);
+        } catch (Throwable t) {
+            throw wrap(t);
+        }
+    }
+
+    /** Attention of new tokens over the paged cache. */
+    public static int pagedAttention(int tokens, int requests, int maxNew, int qHeads, int kvHeads, int headDim, int type, long q, long qStride, long cuNew, long kvLens, long blockTable, int maxPages, int pageSize, int numPages, long kCache, long vCache, float scale, int window, long out, long outStride, long workspace, long workspaceBytes, long stream) {
+        try {
+            return (int) pagedAttention.invokeExact(tokens, requests, maxNew, qHeads, kvHeads, headDim, type, q, qStride, cuNew, kvLens, blockTable, maxPages, pageSize, numPages, kCache, vCache, scale, window, out, outStride, workspace, workspaceBytes, stream);
+        } catch (Throwable t) {
+            throw wrap(t);
+        }
+    }
+
+    /** Workspace of {@link #pagedAttention}. */
+    public static long pagedAttentionWorkspaceBytes(int tokens, int requests, int qHeads, int kvHeads, int headDim) {
+        try {
+            return (long) pagedAttentionWorkspaceBytes.invokeExact(tokens, requests, qHeads, kvHeads, headDim);
         } catch (Throwable t) {
             throw wrap(t);
         }

@@ -142,3 +142,56 @@ def test_rope_of_the_oracle_turns_pairs():
 def test_bf16_patterns_round_to_even():
     assert to_bits(np.float32(1 + 2.0 ** -8), BF16) == 0x3F80 and to_bits(np.float32(1 + 3 * 2.0 ** -8), BF16) == 0x3F82
     assert np.isnan(from_bits(to_bits(np.array([np.nan], np.float32), BF16), BF16))[0]
+
+
+# ---- task factories -----------------------------------------------------------------------------------------------------
+def test_layer_factories_build_descriptors():
+    from tornadovm_b200.arrays import BFloat16Array, ByteArray, FloatArray, HalfFloatArray, Int8Array, IntArray, LongArray
+    from tornadovm_b200.b200 import B200
+    from tornadovm_b200.descriptor import Access
+    x, w, q, s = BFloat16Array(6 * 40), FloatArray(40), Int8Array(240), FloatArray(12)
+    d = B200.addRmsnormQuant(6, 40, x, BFloat16Array(240), w, 1e-5, "int8", 32, q, s)
+    assert d.getFunctionName() == "addRmsnormQuant" and d.getParameters()[2] == 2
+    assert [i for i, a in enumerate(d.getAccess()) if a is not Access.READ_ONLY] == [4, 9, 10] and d.getAccess()[4] is Access.READ_WRITE
+    d = B200.rmsnormQuant(6, 40, FloatArray(240), w, 0.0, "e4m3", 0, ByteArray(240), FloatArray(6))
+    assert d.getParameters()[2] == 0 and d.getParameters()[6:8] == [1, 0]
+    i = lambda n: IntArray(n)  # noqa: E731
+    d = B200.pagedPlan(3, 16, 4, 20, i(3), i(3), i(7), i(12), i(4), i(3), i(20), LongArray(20), i(4))
+    assert d.getParameters()[:5] == [3, 16, 4, 20, 7] and d.getAccess()[8] is Access.READ_WRITE and d.getAccess()[12] is Access.WRITE_ONLY
+    k = HalfFloatArray(5 * 2 * 16 * 64)
+    d = B200.ropeAppend(4, 8, 2, 64, FloatArray(4 * 12 * 64), FloatArray(100 * 32), FloatArray(100 * 32), 64, True, i(4), LongArray(4), 16, HalfFloatArray(4 * 512), k, k)
+    assert d.getParameters()[8:11] == [100, 64, 1] and d.getParameters()[15] == 5
+    d = B200.pagedAttention(4, 3, 2, 8, 2, 64, HalfFloatArray(2048), i(4), i(3), i(12), 16, k, k, 0.125, 0, HalfFloatArray(2048))
+    assert d.getParameters()[11:14] == [4, 16, 5] and d.getAccess()[18] is Access.READ_WRITE
+
+
+def test_layer_factories_refuse_early():
+    from tornadovm_b200.arrays import BFloat16Array, FloatArray, HalfFloatArray, Int8Array, IntArray, LongArray
+    from tornadovm_b200.b200 import B200
+    f, h, i8, i, lo = FloatArray, HalfFloatArray, Int8Array, IntArray, LongArray
+    norm = lambda **k: B200.rmsnormQuant(**(dict(rows=2, cols=64, x=f(128), weight=f(64), eps=1e-5, fmt="int8", group=32, q=i8(128), scales=f(4)) | k))  # noqa: E731
+    norm()
+    for k, text in ((dict(fmt="int4"), "formats"), (dict(group=16), "groups"), (dict(eps=-1.0), "eps"), (dict(scales=f(3)), "too small"), (dict(x=i8(128)), "take")):
+        with pytest.raises(RuntimeError, match=text):
+            norm(**k)
+    with pytest.raises(RuntimeError, match="differ in type"):
+        B200.addRmsnormQuant(2, 64, f(128), h(128), f(64), 1e-5, "int8", 32, i8(128), f(4))
+    with pytest.raises(RuntimeError, match="requests"):
+        B200.pagedPlan(16385, 16, 1, 1, i(1), i(1), i(1), i(1), i(1), i(1), i(1), lo(1), i(4))
+    with pytest.raises(RuntimeError, match="too small"):
+        B200.pagedPlan(2, 16, 1, 1, i(2), i(2), i(1), i(2), i(2), i(2), i(1), lo(1), i(4))
+    k = h(2 * 16 * 64)
+    rope = lambda **a: B200.ropeAppend(**(dict(tokens=1, qHeads=2, kvHeads=2, headDim=64, qkv=f(384), cosTable=f(64), sinTable=f(64), rotDim=64, interleaved=False,  # noqa: E731
+                                               positions=i(1), slots=lo(1), pageSize=16, q=h(128), kCache=k, vCache=k) | a))
+    rope()
+    for a, text in ((dict(rotDim=63), "rotDim"), (dict(kCache=h(100), vCache=h(100)), "whole pages"), (dict(kCache=f(2048), vCache=f(2048)), "take"),
+                    (dict(q=BFloat16Array(128)), "differ in type"), (dict(qkv=f(383)), "too small")):
+        with pytest.raises(RuntimeError, match=text):
+            rope(**a)
+    att = lambda **a: B200.pagedAttention(**(dict(tokens=1, requests=1, maxNew=0, qHeads=4, kvHeads=2, headDim=64, q=h(256), cuNew=i(2), kvLens=i(1), blockTable=i(1),  # noqa: E731
+                                                  pageSize=16, kCache=k, vCache=k, scale=0.1, window=0, out=h(256)) | a))
+    att()
+    for a, text in ((dict(qHeads=3), "multiple of kvHeads"), (dict(scale=0.0), "scale"), (dict(requests=0), "requests"), (dict(out=h(255)), "too small"),
+                    (dict(q=BFloat16Array(256)), "differ in type"), (dict(window=-1), "window")):
+        with pytest.raises(RuntimeError, match=text):
+            att(**a)

@@ -90,3 +90,7 @@ class ByteArray(TornadoNativeArray):
 
 class IntArray(TornadoNativeArray):
     dtype = np.int32
+
+
+class LongArray(TornadoNativeArray):
+    dtype = np.int64

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
-from .arrays import BFloat16Array, ByteArray, FloatArray, HalfFloatArray, Int8Array
+from .arrays import BFloat16Array, ByteArray, FloatArray, HalfFloatArray, Int8Array, IntArray, LongArray
 from .descriptor import Access, LibraryTaskDescriptor
 
 LIBRARY_NAME = "b200/linalg"
@@ -18,6 +18,10 @@ MAX_BATCH = 16
 MAX_GROUP = 32
 #: TaskGraph.libraryTask takes at most 20 arguments (TaskGraph.java:886): rows, cols, batch, x, y, options + 14 matrices
 MAX_GROUP_TASK_ARGS = 14
+#: tb200_type of an array, tb200_quant_format by name (include/tornado_b200.h)
+ELEMENT_TYPES = {FloatArray: 0, HalfFloatArray: 1, BFloat16Array: 2}
+QUANT_FORMATS = {"int8": 0, "e4m3": 1, "e5m2": 2}
+MAX_PLAN_REQUESTS = 16384
 
 
 @dataclass
@@ -43,8 +47,13 @@ def _check(cond: bool, msg: str) -> None:
 
 
 def _desc(function, params, out_index, read_write=False, tuning=None):
+    """``out_index``: the output's place in ``params``, or a dict of the outputs' places and their access."""
     access = [Access.READ_ONLY] * len(params)
-    access[out_index] = Access.READ_WRITE if read_write else Access.WRITE_ONLY
+    if isinstance(out_index, dict):
+        for i, kind in out_index.items():
+            access[i] = kind
+    else:
+        access[out_index] = Access.READ_WRITE if read_write else Access.WRITE_ONLY
     d = LibraryTaskDescriptor().withLibrary(LIBRARY_NAME).withFunction(function).withParameters(params).withAccess(access)
     if tuning is not None:
         d.withTuning(tuning)
@@ -213,3 +222,98 @@ class B200:
         _check(a.getSize() >= batchCount * m * k and b.getSize() >= batchCount * k * n and d.getSize() >= batchCount * m * n,
                "B200 hgemmBatched: array too small")
         return _desc("hgemmBatched", [m, n, k, float(alpha), a, b, float(beta), d, batchCount], 7, read_write=(beta != 0.0))
+
+    # ---- decoder layer: what lies between its quantised products -------------------------------------------
+    @staticmethod
+    def _type(name, array, allowed=(FloatArray, HalfFloatArray, BFloat16Array)):
+        for kind in allowed:
+            if isinstance(array, kind):
+                return ELEMENT_TYPES[kind]
+        raise RuntimeError(f"[ERROR] B200 {name} does not take a {type(array).__name__}")
+
+    @staticmethod
+    def _norm(name, rows, cols, x, residual, weight, eps, fmt, group, q, scales):
+        _check(rows >= 0 and cols >= 1, f"B200 {name} requires rows >= 0 and cols >= 1; got rows={rows}, cols={cols}")
+        _check(fmt in QUANT_FORMATS, f"B200 {name} knows the formats {', '.join(QUANT_FORMATS)}; got {fmt}")
+        _check(group in (0, 32, 64, 128), f"B200 {name} requires groups of 32, 64 or 128 columns, or 0 for a scale per row; got {group}")
+        _check(0.0 <= eps < float("inf"), f"B200 {name} requires a finite eps >= 0; got {eps}")
+        groups = -(-cols // group) if group else 1
+        _check(x.getSize() >= rows * cols and weight.getSize() >= cols and q.getSize() >= rows * cols and scales.getSize() >= rows * groups
+               and (residual is None or residual.getSize() >= rows * cols), f"B200 {name}: array too small")
+        kind = B200._type(name, x)
+        _check(residual is None or type(residual) is type(x), f"B200 {name}: x and residual differ in type")
+        arrays = [x] if residual is None else [x, residual]
+        params = [rows, cols, kind, *arrays, weight, float(eps), QUANT_FORMATS[fmt], group, q, scales]
+        out = {len(params) - 2: Access.WRITE_ONLY, len(params) - 1: Access.WRITE_ONLY}
+        if residual is not None:
+            out[4] = Access.READ_WRITE
+        return _desc(name, params, out)
+
+    @staticmethod
+    def rmsnormQuant(rows, cols, x, weight: FloatArray, eps, fmt, group, q, scales: FloatArray):  # noqa: N802
+        """Root-mean-square norm of x's rows times ``weight`` as 8-bit values (``fmt``: int8, e4m3, e5m2) with an fp32
+        scale per ``group`` columns (0: per row): the rows of A for igemm / fp8gemm, or the int8 blocks of the mat-vecs."""
+        return B200._norm("rmsnormQuant", rows, cols, x, None, weight, eps, fmt, group, q, scales)
+
+    @staticmethod
+    def addRmsnormQuant(rows, cols, x, residual, weight: FloatArray, eps, fmt, group, q, scales: FloatArray):  # noqa: N802
+        """rmsnormQuant of ``residual + x``; the sum, rounded to the arrays' type, replaces ``residual``."""
+        return B200._norm("addRmsnormQuant", rows, cols, x, residual, weight, eps, fmt, group, q, scales)
+
+    @staticmethod
+    def pagedPlan(requests, pageSize, maxPages, maxTokens, cachedLens: IntArray, newLens: IntArray, freePages: IntArray,  # noqa: N802,N803
+                  blockTable: IntArray, cuNew: IntArray, kvLens: IntArray, positions: IntArray, slots: LongArray, counts: IntArray):  # noqa: N803
+        """Lays out a step of a paged cache: fresh pages from ``freePages`` into the table rows, and each token row's
+        position and slot (tb200_paged_plan)."""
+        _check(0 <= requests <= MAX_PLAN_REQUESTS, f"B200 pagedPlan requires 0 <= requests <= {MAX_PLAN_REQUESTS}; got {requests}")
+        _check(pageSize >= 1 and maxPages >= 0 and maxPages * pageSize <= 1 << 30, "B200 pagedPlan requires pages of at least one position and at most 2^30 positions in a table row")
+        _check(0 <= maxTokens <= 1 << 30, f"B200 pagedPlan requires 0 <= maxTokens <= 2^30; got {maxTokens}")
+        _check(cachedLens.getSize() >= requests and newLens.getSize() >= requests and blockTable.getSize() >= requests * maxPages
+               and cuNew.getSize() >= requests + 1 and kvLens.getSize() >= requests and positions.getSize() >= maxTokens
+               and slots.getSize() >= maxTokens and counts.getSize() >= 4, "B200 pagedPlan: array too small")
+        params = [requests, pageSize, maxPages, maxTokens, freePages.getSize(), cachedLens, newLens, freePages, blockTable, cuNew, kvLens, positions, slots, counts]
+        return _desc("pagedPlan", params, {8: Access.READ_WRITE} | {i: Access.WRITE_ONLY for i in range(9, 14)})
+
+    @staticmethod
+    def _cache(name, kvHeads, headDim, pageSize, kCache, vCache):  # noqa: N803
+        _check(kvHeads >= 1 and headDim >= 1 and pageSize >= 1, f"B200 {name} requires kvHeads, headDim and pageSize >= 1")
+        per = kvHeads * pageSize * headDim
+        _check(kCache.getSize() == vCache.getSize() and kCache.getSize() % per == 0,
+               f"B200 {name}: the caches are not both whole pages of kvHeads x pageSize x headDim = {per} elements")
+        kind = B200._type(name, kCache, (HalfFloatArray, BFloat16Array))
+        _check(type(vCache) is type(kCache), f"B200 {name}: the caches differ in type")
+        return kind, kCache.getSize() // per
+
+    @staticmethod
+    def ropeAppend(tokens, qHeads, kvHeads, headDim, qkv, cosTable: FloatArray, sinTable: FloatArray, rotDim, interleaved, positions: IntArray,  # noqa: N802,N803
+                   slots: LongArray, pageSize, q, kCache, vCache):  # noqa: N803
+        """Rotates the queries and keys of projection rows [tokens][(qHeads + 2 kvHeads) headDim] by their positions,
+        stores the queries in ``q`` and keys and values at their slots of the cache (tb200_rope_append)."""
+        kind, pages = B200._cache("ropeAppend", kvHeads, headDim, pageSize, kCache, vCache)
+        _check(tokens >= 0 and qHeads >= 0, f"B200 ropeAppend requires tokens >= 0 and qHeads >= 0; got {tokens}, {qHeads}")
+        _check(0 <= rotDim <= headDim and rotDim % 2 == 0, f"B200 ropeAppend requires an even rotDim of at most headDim; got {rotDim}")
+        rows = min(cosTable.getSize(), sinTable.getSize()) // (rotDim // 2) if rotDim else 0
+        _check(qkv.getSize() >= tokens * (qHeads + 2 * kvHeads) * headDim and q.getSize() >= tokens * qHeads * headDim
+               and positions.getSize() >= tokens and slots.getSize() >= tokens, "B200 ropeAppend: array too small")
+        _check(type(q) is type(kCache), "B200 ropeAppend: q and the caches differ in type")
+        params = [tokens, qHeads, kvHeads, headDim, B200._type("ropeAppend", qkv), qkv, cosTable, sinTable, rows, rotDim, int(bool(interleaved)), positions,
+                  kind, q, pageSize, pages, slots, kCache, vCache]
+        return _desc("ropeAppend", params, {i: Access.READ_WRITE for i in (13, 17, 18)})
+
+    @staticmethod
+    def pagedAttention(tokens, requests, maxNew, qHeads, kvHeads, headDim, q, cuNew: IntArray, kvLens: IntArray, blockTable: IntArray,  # noqa: N802,N803
+                       pageSize, kCache, vCache, scale, window, out):  # noqa: N803
+        """Causal attention of each request's new tokens over its pages of the cache, the new tokens included
+        (tb200_paged_attention); ``window`` 0: no limit, ``maxNew`` 0: no bound known."""
+        kind, pages = B200._cache("pagedAttention", kvHeads, headDim, pageSize, kCache, vCache)
+        _check(tokens >= 0 and requests >= 1 and maxNew >= 0 and window >= 0, "B200 pagedAttention requires tokens, maxNew, window >= 0 and requests >= 1")
+        _check(qHeads >= kvHeads and qHeads % kvHeads == 0, f"B200 pagedAttention requires qHeads to be a multiple of kvHeads; got {qHeads}, {kvHeads}")
+        _check(headDim % 8 == 0 and headDim <= 256, f"B200 pagedAttention requires headDim to be a multiple of 8 up to 256; got {headDim}")
+        _check(0.0 < scale < float("inf"), f"B200 pagedAttention requires a finite scale > 0; got {scale}")
+        _check(blockTable.getSize() % requests == 0 and blockTable.getSize() // requests * pageSize <= 1 << 30, "B200 pagedAttention: the table is not [requests][maxPages], or a row holds over 2^30 positions")
+        _check(q.getSize() >= tokens * qHeads * headDim and out.getSize() >= tokens * qHeads * headDim and cuNew.getSize() >= requests + 1
+               and kvLens.getSize() >= requests, "B200 pagedAttention: array too small")
+        _check(type(q) is type(kCache) and type(out) is type(kCache), "B200 pagedAttention: q, out and the caches differ in type")
+        params = [tokens, requests, maxNew, qHeads, kvHeads, headDim, kind, q, cuNew, kvLens, blockTable, blockTable.getSize() // requests, pageSize, pages,
+                  kCache, vCache, float(scale), window, out]
+        return _desc("pagedAttention", params, {18: Access.READ_WRITE})

@@ -112,7 +112,7 @@ class B200LibraryProvider:
     _PREPARE_CLASS = {"sgemv": 1, "q8Gemv": 2, "q8GemvBytes": 2, "q4GemvBytes": 2, "q8GemvBytesGrouped": 2,
                       "q4GemvBytesGrouped": 2, "q8GemvBytesPacked": 2, "q4GemvBytesPacked": 2, "sgemm": 4, "hgemmF32": 8, "hgemm": 8, "bgemm": 8, "hgemmBatched": 8,
                       "gemmBiasRelu": 8, "gemmBiasGelu": 8, "gemmBiasSilu": 8, "gemmBiasSigmoid": 8, "gemmBiasTanh": 8,
-                      "gemmBiasHardSwish": 8}
+                      "gemmBiasHardSwish": 8, "rmsnormQuant": 32, "addRmsnormQuant": 32, "pagedPlan": 32, "ropeAppend": 32, "pagedAttention": 32}
 
     def prepare(self, descriptor, context: B200Context) -> None:
         """Runs in the pre-launch pass, before any capture (TornadoVMInterpreter.java:1036-1055) and possibly
@@ -129,6 +129,9 @@ class B200LibraryProvider:
         if fn in _PACKED_FUNCTIONS:  # (count, rows, cols, batch, blocks, x, y)
             p = descriptor.getParameters()
             context.grow_workspace(int(B200Native.load().tb200_qx_workspace_bytes(int(p[2]), int(p[3]))))
+        if fn == "pagedAttention":  # (tokens, requests, maxNew, qHeads, kvHeads, headDim, ...)
+            p = descriptor.getParameters()
+            context.grow_workspace(int(B200Native.load().tb200_paged_attention_workspace_bytes(p[0], p[1], p[3], p[4], p[5])))
         if fn in _GROUPED_FUNCTIONS:  # (count, rows, cols, batch, x, y, blocks...); integer mode whatever the tuning says
             p = descriptor.getParameters()
             context.grow_workspace(int(B200Native.load().tb200_qx_workspace_bytes(int(p[2]), int(p[3]))))
@@ -195,6 +198,25 @@ class B200LibraryProvider:
         elif functionName in _BIAS_ACTIVATIONS:  # (m, n, k, a, b, bias, d): fp16 in and out
             st = lib.tb200_gemm_ex(A(0), A(1), A(2), 0, P(3), P(4), 1, P(6), 1.0, 0.0, None, P(5), _BIAS_ACTIVATIONS[functionName], 1,
                                    ctx.stream)
+        elif functionName == "rmsnormQuant":  # (rows, cols, type, x, weight, eps, format, group, q, scales)
+            st = lib.tb200_rmsnorm_quant(A(0), A(1), A(2), P(3), A(1), None, None, P(4), A(5), A(6), A(7), P(8), P(9), ctx.stream)
+        elif functionName == "addRmsnormQuant":  # (rows, cols, type, x, residual, weight, eps, format, group, q, scales)
+            st = lib.tb200_rmsnorm_quant(A(0), A(1), A(2), P(3), A(1), P(4), P(4), P(5), A(6), A(7), A(8), P(9), P(10), ctx.stream)
+        elif functionName == "pagedPlan":  # (requests, pageSize, maxPages, maxTokens, numFree, nine arrays)
+            st = lib.tb200_paged_plan(*[A(i) for i in range(5)], *[P(i) for i in range(5, 14)], ctx.stream)
+        elif functionName == "ropeAppend":
+            # (tokens, qHeads, kvHeads, headDim, inType, qkv, cos, sin, tableRows, rotDim, interleaved, positions, cacheType, q, pageSize, numPages,
+            #  slots, kCache, vCache): queries, keys and values of a token lie in one row
+            size = 4 if A(4) == 0 else 2
+            row, k = (A(1) + 2 * A(2)) * A(3), A(1) * A(3) * size
+            st = lib.tb200_rope_append(A(0), A(1), A(2), A(3), A(4), P(5), P(5) + k, P(5) + k + A(2) * A(3) * size, row, row, row, P(6), P(7), A(8), A(9), A(10),
+                                       P(11), A(12), P(13), A(14), A(15), P(16), P(17), P(18), ctx.stream)
+        elif functionName == "pagedAttention":
+            # (tokens, requests, maxNew, qHeads, kvHeads, headDim, type, q, cuNew, kvLens, blockTable, maxPages, pageSize, numPages, kCache, vCache,
+            #  scale, window, out)
+            row = A(3) * A(5)
+            st = lib.tb200_paged_attention(*[A(i) for i in range(7)], P(7), row, P(8), P(9), P(10), A(11), A(12), A(13), P(14), P(15), A(16), A(17), P(18), row,
+                                           *ws, ctx.stream)
         else:
             raise RuntimeError(f"[ERROR] B200 function not supported: {functionName}")
         return st
