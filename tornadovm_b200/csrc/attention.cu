@@ -19,7 +19,7 @@ namespace tb200 {
 
 constexpr int AT_THREADS = 128, AT_KEYS = 64;
 constexpr int AT_ITEM = 1;       // what an item costs besides its key tiles, in such tiles
-constexpr int AT_TC_ROWS = 64;   // requests of more rows go to the tensor-memory kernel
+constexpr int AT_TC_ROWS = 16;   // requests of more rows go to the tensor-memory kernel (45 requests of 32 rows over 3420 keys: 108 us there, 193 us here)
 constexpr int AT_MAX_SMS = 148;  // the workspace is sized without asking the device
 
 __device__ __forceinline__ float ex2(float x) {

@@ -229,12 +229,14 @@ struct AttnWalk {
 };
 
 // Joins the parts of the items that more than one block worked on.  Block x takes the item that block x of the main
-// kernel began and another one ended; the rows of the tile are spread over gridDim.y.  Each of the four warps takes
-// every fourth part; a lane holds DPAD / 32 columns.
+// kernel began and another one ended; the rows of the tile are spread over gridDim.y.  A long context has hundreds of
+// parts, so their maxima and sums are read side by side first, a part a thread, and become weights in shared memory;
+// then each of the four warps adds up every fourth part, a lane DPAD / 32 columns, with no read waiting for another.
+constexpr int JOIN_PARTS = 512;  // weights held at a time
 template <class T, int ROWS, int DPAD>
 __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
     constexpr int PITCH = DPAD + 2, COLS = DPAD / 32;
-    __shared__ float acc_s[4][DPAD], ml_s[4][2];
+    __shared__ float acc_s[4][DPAD], weight[JOIN_PARTS], red[4][2];
     pdl_wait();
     const int4 item = a.joins[blockIdx.x];
     if (item.x < 0) return;
@@ -242,46 +244,52 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
     const int rows = min(ROWS, q.rows - item.z * ROWS), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int parts = item.w - (int)blockIdx.x + 1;
     for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-        float m = -INFINITY, l = 0.0f, acc[COLS] = {};
-        for (int i = warp; i < parts; i += 4) {
-            const float *p = a.parts + (((long long)(blockIdx.x + i) * 2 + (i == 0)) * ROWS + row) * PITCH;
-            const float pm = p[DPAD], pl = p[DPAD + 1];
-            float v[COLS];
-#pragma unroll
-            for (int c = 0; c < COLS; c += 2) {
-                const float2 f = *reinterpret_cast<const float2 *>(p + lane * COLS + c);
-                v[c] = f.x, v[c + 1] = f.y;
-            }
-            if (pl == 0.0f) continue;  // a part that saw nothing
-            const float top = fmaxf(m, pm), w0 = exp2f(m - top), w1 = exp2f(pm - top);
-            l = l * w0 + pl * w1;
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) acc[c] = acc[c] * w0 + v[c] * w1;
-            m = top;
+        // part i: block x + i, in the place for an item that it began (the first one) or found begun
+        auto part = [&](int i) { return a.parts + (((long long)(blockIdx.x + i) * 2 + (i == 0)) * ROWS + row) * PITCH; };
+        float top = -INFINITY;
+        for (int i = threadIdx.x; i < parts; i += 128) {
+            const float2 ml = *reinterpret_cast<const float2 *>(part(i) + DPAD);
+            if (ml.y != 0.0f) top = fmaxf(top, ml.x);  // a part that saw nothing has the sum 0
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         __syncthreads();
-        if (lane == 0) ml_s[warp][0] = m, ml_s[warp][1] = l;
+        if (lane == 0) red[warp][0] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+        float sum = 0.0f, acc[COLS] = {};
+        for (int p0 = 0; p0 < parts; p0 += JOIN_PARTS) {
+            const int n = min(JOIN_PARTS, parts - p0);
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += 128) {
+                const float2 ml = *reinterpret_cast<const float2 *>(part(p0 + i) + DPAD);
+                const float w = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top);
+                weight[i] = w;
+                sum += ml.y * w;
+            }
+            __syncthreads();
+#pragma unroll 4
+            for (int i = warp; i < n; i += 4) {
+                const float w = weight[i];
+                const float *v = part(p0 + i) + lane * COLS;
+#pragma unroll
+                for (int c = 0; c < COLS; c += 2) {
+                    const float2 f = *reinterpret_cast<const float2 *>(v + c);
+                    if (w != 0.0f) acc[c] += f.x * w, acc[c + 1] += f.y * w;
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) red[warp][1] = sum;
 #pragma unroll
         for (int c = 0; c < COLS; ++c) acc_s[warp][lane * COLS + c] = acc[c];
         __syncthreads();
-        float top = -INFINITY, sum = 0.0f, w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = ml_s[i][1] == 0.0f ? top : fmaxf(top, ml_s[i][0]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = ml_s[i][1] == 0.0f ? 0.0f : exp2f(ml_s[i][0] - top);
-            sum += ml_s[i][1] * w[i];
-        }
+        sum = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int at = item.z * ROWS + row, token = at / a.group, head = item.y * a.group + at % a.group;
         T *dst = static_cast<T *>(a.out) + (q.first + token) * a.out_stride + (long long)head * a.head_dim;
-        for (int d = threadIdx.x; d < a.head_dim; d += 128) {
-            float v = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (w[i] != 0.0f) v += acc_s[i][d] * w[i];
-            from_f32(dst[d], v * inv);
-        }
+        for (int d = threadIdx.x; d < a.head_dim; d += 128) from_f32(dst[d], ((acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d])) * inv);
     }
 }
 
