@@ -20,6 +20,7 @@ namespace tb200 {
 constexpr int AT_THREADS = 128, AT_KEYS = 64;
 constexpr int AT_ITEM = 1;       // what an item costs besides its key tiles, in such tiles
 constexpr int AT_TC_ROWS = 16;   // requests of more rows go to the tensor-memory kernel (45 requests of 32 rows over 3420 keys: 108 us there, 193 us here)
+constexpr int AT_WHOLE_TILES = 4;  // contexts of up to this many key tiles are not split
 constexpr int AT_MAX_SMS = 148;  // the workspace is sized without asking the device
 
 __device__ __forceinline__ float ex2(float x) {
@@ -68,7 +69,7 @@ struct AtShape {
     static constexpr int RING = STAGES + 1;  // tiles whose rows have been looked up
     static constexpr int SMEM = Q_BYTES + STAGES * 2 * TILE_BYTES + RING * AT_KEYS * 8 + RING * 2 * 4;
     static constexpr int GRID = AT_MAX_SMS * BLOCKS_PER_SM;
-    static constexpr size_t PART_FLOATS = (size_t)ROWS * (DPAD + 2);
+    static constexpr size_t PART_FLOATS = (size_t)ROWS * attn_part_pitch(DPAD);
     static constexpr size_t WORKSPACE = GRID * sizeof(int4) + GRID * 2 * PART_FLOATS * 4;
     static_assert(!SPLIT_KEYS || STAGES * 2 * TILE_BYTES >= 4 * 16 * (DPAD + 2) * 4, "the warps' results fit the drained stages");
 };
@@ -95,14 +96,16 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
     const long long v_ahead = static_cast<const char *>(a.v_cache) - static_cast<const char *>(a.k_cache);
     const bool copy16 = ((uintptr_t)a.k_cache & 15) == 0 && ((uintptr_t)a.v_cache & 15) == 0;
 
-    attn_find_start<AT_THREADS, ROWS, AT_KEYS, AT_ITEM>(a, &start, scan);
-    if (start.begin >= start.end) {
-        if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-        pdl_launch_dependents();
-        return;
+    if (!a.whole) {
+        attn_find_start<AT_THREADS, ROWS, AT_KEYS, AT_ITEM>(a, &start, scan);
+        if (start.begin >= start.end) {
+            if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+            pdl_launch_dependents();
+            return;
+        }
     }
     AttnWalk<ROWS, AT_KEYS, AT_ITEM> w;
-    bool more = w.seek(a, start);
+    bool more = a.whole ? w.first_whole(a) : w.seek(a, start);
     int4 join = make_int4(-1, 0, 0, 0);
 
     while (more) {
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
                     from_f32(dst[1], y * inv);
                 }
             } else {
-                *reinterpret_cast<float2 *>(part + row * (DPAD + 2) + d) = make_float2(x, y);
+                *reinterpret_cast<float2 *>(part + row * attn_part_pitch(DPAD) + d) = make_float2(x, y);
             }
         };
         if constexpr (SPLIT_KEYS) {
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
                     sum += v.y * f, x += c.x * f, y += c.y * f;
                 }
                 put(row, d, x, y, sum == 0.0f ? 0.0f : 1.0f / sum);
-                if (!whole && d == 0) part[row * (DPAD + 2) + DPAD] = top, part[row * (DPAD + 2) + DPAD + 1] = sum;
+                if (!whole && d == 0) part[row * attn_part_pitch(DPAD) + DPAD] = top, part[row * attn_part_pitch(DPAD) + DPAD + 1] = sum;
             }
         } else {
 #pragma unroll
@@ -402,12 +405,13 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
                     const float inv = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
 #pragma unroll
                     for (int n = 0; n < DPAD / 8; ++n) put(row, 8 * n + 2 * (lane & 3), o[n][2 * h], o[n][2 * h + 1], inv);
-                    if (!whole && (lane & 3) == 0) part[row * (DPAD + 2) + DPAD] = m[h], part[row * (DPAD + 2) + DPAD + 1] = l[h];
+                    if (!whole && (lane & 3) == 0) part[row * attn_part_pitch(DPAD) + DPAD] = m[h], part[row * attn_part_pitch(DPAD) + DPAD + 1] = l[h];
                 }
             }
         }
-        more = w.next(a, start);
+        more = a.whole ? w.next_whole(a) : w.next(a, start);
     }
+    if (a.whole) return;
     if (tid == 0) a.joins[blockIdx.x] = join;
     pdl_launch_dependents();
 }
@@ -422,13 +426,21 @@ static int attn_launch(AttnArgs a, int longest_rows, void *workspace, const Devi
     if (st) return st;
     st = ensure_kernel<attn_join_kernel<T, S::ROWS, DPAD>, 0>(di);
     if (st) return st;
-    const int grid = min(di->sm_count, AT_MAX_SMS) * S::BLOCKS_PER_SM;
+    int grid = min(di->sm_count, AT_MAX_SMS) * S::BLOCKS_PER_SM;
+    // Short contexts: the search for a block's share and the join take longer than a whole item does.  Six requests of 157
+    // keys: 16.4 us split, 12.0 us whole; eight of 500 keys: 15.5 us split, 19.9 us whole.
+    const long long keys = min((long long)a.max_pages * a.page_size, a.window > 0 ? (long long)a.window + longest_rows / a.group : 1LL << 40);
+    a.whole = keys <= AT_WHOLE_TILES * AT_KEYS && (long long)a.requests * a.kv_heads <= 0x3FFFFFFF;
+    if (a.whole) {
+        grid = (int)min((long long)grid, (long long)a.requests * a.kv_heads);
+        return launch_kernel(attn_kernel<T, DPAD, SPLIT_KEYS>, dim3(grid), dim3(AT_THREADS), S::SMEM, s, false, a);
+    }
     a.joins = static_cast<int4 *>(workspace);
     a.parts = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + S::GRID * sizeof(int4));
     st = launch_kernel(attn_kernel<T, DPAD, SPLIT_KEYS>, dim3(grid), dim3(AT_THREADS), S::SMEM, s, false, a);
     if (st) return st;
     // the join waits for the main kernel by itself (programmatic launch): its start-up is hidden behind it
-    return launch_kernel(attn_join_kernel<T, S::ROWS, DPAD>, dim3(grid, min(longest_rows, S::ROWS)), dim3(128), 0, s, true, a);
+    return launch_kernel(attn_join_kernel<T, S::ROWS, DPAD>, dim3(grid, min(longest_rows, 8)), dim3(JOIN_WARPS * 32), 0, s, true, a);
 }
 
 template <class T, int DPAD>
@@ -492,7 +504,6 @@ extern "C" int tb200_paged_attention(int tokens, int requests, int max_new, int 
     a.tokens = tokens, a.requests = requests, a.q_heads = q_heads, a.kv_heads = kv_heads, a.group = q_heads / kv_heads, a.head_dim = head_dim;
     a.max_pages = max_pages, a.page_size = page_size, a.num_pages = num_pages, a.window = window;
     a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
-    a.min_rows = 1, a.max_rows = 0x7FFFFFFF;
     const long long longest = (long long)(max_new > 0 ? min(max_new, tokens) : tokens) * a.group;
     const int rows = (int)min(longest, 0x7FFFFFFFLL);
     if (rows > AT_TC_ROWS && attn_tc_eligible(a)) return attn_tc_launch(a, type, rows, workspace, di, (cudaStream_t)stream);

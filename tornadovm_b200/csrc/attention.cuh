@@ -24,12 +24,12 @@ struct AttnArgs {
     const void *q, *k_cache, *v_cache;
     const int32_t *cu_new, *kv_lens, *block_table;
     void *out;
-    float *parts;        // [grid][2][rows of a tile][DPAD + 2 floats]: output, then maximum and sum
+    float *parts;        // [grid][2][rows of a tile][pitch]: output, then maximum and sum
     int4 *joins;         // [grid]: item that the block begins and another one ends: (request, kv head, row tile, last block), x < 0: none
     long long q_stride, out_stride;
     float scale_log2;    // scale * log2(e): probabilities are powers of two
     int tokens, requests, q_heads, kv_heads, group, head_dim, max_pages, page_size, num_pages, window, page_shift;  // page_shift: log2, or -1
-    int min_rows, max_rows;  // only requests with min_rows <= rows <= max_rows are this kernel's
+    int whole;  // items are not split: every gridDim.x-th (request, kv head) belongs to a block
 };
 
 struct AttnRequest {
@@ -43,7 +43,7 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnArgs &a, int r) {
     const int b = min(max(a.cu_new[r], 0), a.tokens), e = min(max(a.cu_new[r + 1], b), a.tokens);
     q.first = b, q.new_tokens = e - b;
     const long long rows = (long long)q.new_tokens * a.group;
-    q.rows = rows >= a.min_rows && rows <= a.max_rows ? (int)rows : 0;
+    q.rows = (int)rows;
     q.kv_len = min(max(a.kv_lens[r], 0), 1 << 30);
     q.visible = (int)min((long long)q.kv_len, (long long)a.max_pages * a.page_size);
     return q;
@@ -225,18 +225,39 @@ struct AttnWalk {
         attn_key_tiles<ROWS, KEYS>(a, q, tile, first, count);
         return clip(s);  // only the block's last item can be without key tiles of it
     }
+    // The walk over whole items: row tiles of (request, kv head) `pair`, of every gridDim.x-th pair from there on.
+    int pair;
+    __device__ __forceinline__ bool first_whole(const AttnArgs &a) {
+        pair = (int)blockIdx.x - (int)gridDim.x, tile = 0, q.rows = 0;
+        return next_whole(a);
+    }
+    __device__ __forceinline__ bool next_whole(const AttnArgs &a) {
+        ++tile;
+        while ((long long)tile * ROWS >= q.rows) {
+            if ((long long)pair + gridDim.x >= (long long)a.requests * a.kv_heads) return false;
+            pair += gridDim.x, tile = 0;
+            request = pair / a.kv_heads, head = pair - request * a.kv_heads;
+            q = attn_request(a, request);
+        }
+        attn_key_tiles<ROWS, KEYS>(a, q, tile, first, count);
+        from = 0, to = count;
+        return true;
+    }
     __device__ __forceinline__ bool whole() const { return from == 0 && to == count; }
 };
 
 // Joins the parts of the items that more than one block worked on.  Block x takes the item that block x of the main
 // kernel began and another one ended; the rows of the tile are spread over gridDim.y.  A long context has hundreds of
 // parts, so their maxima and sums are read side by side first, a part a thread, and become weights in shared memory;
-// then each of the four warps adds up every fourth part, a lane DPAD / 32 columns, with no read waiting for another.
+// then each of the eight warps adds up every eighth part, a lane DPAD / 32 columns, with eight reads under way at once.
 constexpr int JOIN_PARTS = 512;  // weights held at a time
+constexpr int JOIN_WARPS = 8;
+// floats of a row of a part: the output, the maximum, the sum, and what keeps rows at 16 bytes
+__host__ __device__ constexpr int attn_part_pitch(int dpad) { return dpad + 4; }
 template <class T, int ROWS, int DPAD>
-__global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
-    constexpr int PITCH = DPAD + 2, COLS = DPAD / 32;
-    __shared__ float acc_s[4][DPAD], weight[JOIN_PARTS], red[4][2];
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attn_join_kernel(AttnArgs a) {
+    constexpr int PITCH = attn_part_pitch(DPAD), COLS = DPAD / 32, THREADS = JOIN_WARPS * 32;
+    __shared__ float acc_s[JOIN_WARPS][DPAD], weight[JOIN_PARTS], red[JOIN_WARPS][2];
     pdl_wait();
     const int4 item = a.joins[blockIdx.x];
     if (item.x < 0) return;
@@ -247,7 +268,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
         // part i: block x + i, in the place for an item that it began (the first one) or found begun
         auto part = [&](int i) { return a.parts + (((long long)(blockIdx.x + i) * 2 + (i == 0)) * ROWS + row) * PITCH; };
         float top = -INFINITY;
-        for (int i = threadIdx.x; i < parts; i += 128) {
+        for (int i = threadIdx.x; i < parts; i += THREADS) {
             const float2 ml = *reinterpret_cast<const float2 *>(part(i) + DPAD);
             if (ml.y != 0.0f) top = fmaxf(top, ml.x);  // a part that saw nothing has the sum 0
         }
@@ -256,20 +277,21 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
         __syncthreads();
         if (lane == 0) red[warp][0] = top;
         __syncthreads();
-        top = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; ++w) top = fmaxf(top, red[w][0]);
         float sum = 0.0f, acc[COLS] = {};
         for (int p0 = 0; p0 < parts; p0 += JOIN_PARTS) {
             const int n = min(JOIN_PARTS, parts - p0);
             __syncthreads();
-            for (int i = threadIdx.x; i < n; i += 128) {
+            for (int i = threadIdx.x; i < n; i += THREADS) {
                 const float2 ml = *reinterpret_cast<const float2 *>(part(p0 + i) + DPAD);
                 const float w = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top);
                 weight[i] = w;
                 sum += ml.y * w;
             }
             __syncthreads();
-#pragma unroll 4
-            for (int i = warp; i < n; i += 4) {
+#pragma unroll 8
+            for (int i = warp; i < n; i += JOIN_WARPS) {
                 const float w = weight[i];
                 const float *v = part(p0 + i) + lane * COLS;
 #pragma unroll
@@ -285,11 +307,18 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a) {
 #pragma unroll
         for (int c = 0; c < COLS; ++c) acc_s[warp][lane * COLS + c] = acc[c];
         __syncthreads();
-        sum = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; ++w) sum += red[w][1];
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int at = item.z * ROWS + row, token = at / a.group, head = item.y * a.group + at % a.group;
         T *dst = static_cast<T *>(a.out) + (q.first + token) * a.out_stride + (long long)head * a.head_dim;
-        for (int d = threadIdx.x; d < a.head_dim; d += 128) from_f32(dst[d], ((acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d])) * inv);
+        for (int d = threadIdx.x; d < a.head_dim; d += THREADS) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < JOIN_WARPS; ++w) v += acc_s[w][d];
+            from_f32(dst[d], v * inv);
+        }
     }
 }
 
