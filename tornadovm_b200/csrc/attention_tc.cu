@@ -1,7 +1,7 @@
 // Attention of chunks of new tokens over a paged cache on the 5th-generation tensor cores.
 //
-// One persistent block per SM works on tiles of 256 query rows (two of 128, one per lane of tensor memory) against key
-// tiles of 64:
+// One persistent block per SM works on tiles of 256 query rows (two of 128, a row per lane of tensor memory; one with heads
+// of more than 128 columns) against key tiles of 64:
 //   * warp 8 fetches K and V tiles into two rings of shared-memory slots, one TMA box per page and 64 columns (lanes look
 //     the pages up side by side, a tile ahead); a page that no row sees, or that is none of the cache's, is fetched from
 //     behind the end of the tensor map and arrives as zeros;
@@ -30,7 +30,7 @@ namespace tb200 {
 
 // An item costs its block about as much beside its key tiles (edge tiles, the rows' store) as this many of them.
 constexpr int TC_ITEM = 8;
-constexpr int TC_ROWS = 256, TC_KEYS = 64, TC_THREADS = 384;  // three warpgroups
+constexpr int TC_KEYS = 64, TC_THREADS = 384;  // three warpgroups
 // Registers: 384 threads are launched with 168 each, which the softmax threads (64 scores and 32 words of P in registers) outgrow, so the
 // warpgroups share them anew: 2 * 192 + 120 = 3 * 168.
 constexpr int TC_SOFTMAX_REGS = 192, TC_OTHER_REGS = 120;
@@ -38,13 +38,14 @@ static_assert(2 * TC_SOFTMAX_REGS + TC_OTHER_REGS == 3 * 168, "the shares add up
 
 template <int DPAD>
 struct TcShape {
+    static constexpr int TILES = DPAD == 256 ? 1 : 2, ROWS = 128 * TILES;  // 256 columns fill tensor and shared memory with one row tile
     static constexpr int PANELS = DPAD / 64;  // 64 columns = 128 bytes: the swizzled rows of a tile
     static constexpr int KV_PANEL = TC_KEYS * 128, KV_BYTES = PANELS * KV_PANEL;   // K or V tile
     static constexpr int Q_PANEL = 128 * 128, Q_BYTES = PANELS * Q_PANEL;          // 128 query rows
-    static constexpr int SLOTS = DPAD == 128 ? 5 : 10;                             // each a K and a V tile
-    static constexpr int SMEM = 2 * Q_BYTES + 2 * SLOTS * KV_BYTES + 1024;
+    static constexpr int SLOTS = DPAD == 256 ? 2 : DPAD == 128 ? 5 : 10;           // each a K and a V tile
+    static constexpr int SMEM = TILES * Q_BYTES + 2 * SLOTS * KV_BYTES + 1024;
     static constexpr int GRID = 148;
-    static constexpr size_t PART_FLOATS = (size_t)TC_ROWS * (DPAD + 2);
+    static constexpr size_t PART_FLOATS = (size_t)ROWS * (DPAD + 2);
     static constexpr size_t WORKSPACE = GRID * sizeof(int4) + GRID * 2 * PART_FLOATS * 4;
     // tensor memory: two score buffers of 64 columns for each row tile (P in the first 32 of a buffer), then O_0 and O_1
     static constexpr uint32_t O_COL = 256, TMEM_COLS = 512;
@@ -108,10 +109,12 @@ __device__ __forceinline__ void tc_store8(T *dst, const uint32_t (&h)[4], uintpt
 }
 
 // What the rows of an item see.
+template <int DPAD>
 struct TcItem {
+    static constexpr int ROWS = TcShape<DPAD>::ROWS;
     int row0, rows, base, pos_first, pos_last, key_lo, key_hi, tile0, ntiles;
-    __device__ __forceinline__ TcItem(const AttnArgs &a, const AttnWalk<TC_ROWS, TC_KEYS, TC_ITEM> &w) {
-        row0 = w.tile * TC_ROWS, rows = min(TC_ROWS, w.q.rows - row0), base = w.q.kv_len - w.q.new_tokens;
+    __device__ __forceinline__ TcItem(const AttnArgs &a, const AttnWalk<ROWS, TC_KEYS, TC_ITEM> &w) {
+        row0 = w.tile * ROWS, rows = min(ROWS, w.q.rows - row0), base = w.q.kv_len - w.q.new_tokens;
         pos_first = base + row0 / a.group, pos_last = base + (row0 + rows - 1) / a.group;
         key_lo = a.window > 0 ? max(0, pos_first - a.window + 1) : 0, key_hi = min(pos_last, w.q.visible - 1);
         tile0 = w.first + w.from, ntiles = w.to - w.from;
@@ -123,11 +126,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a, uint32_t idesc_qk,
                uint32_t idesc_pv) {
     using S = TcShape<DPAD>;
-    constexpr int PANELS = S::PANELS, SLOTS = S::SLOTS;
+    constexpr int PANELS = S::PANELS, SLOTS = S::SLOTS, ROWS = S::ROWS;
     extern __shared__ __align__(128) unsigned char tc_smem[];
     __shared__ __align__(16) TcShared sh;
     unsigned char *q_s = reinterpret_cast<unsigned char *>(((uintptr_t)tc_smem + 1023) & ~(uintptr_t)1023);  // swizzled tiles: 1024-byte bases
-    unsigned char *kv_s = q_s + 2 * S::Q_BYTES;  // slot: K tile, V tile
+    unsigned char *kv_s = q_s + S::TILES * S::Q_BYTES;  // slot: K tile, V tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -140,7 +143,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         mbar_fence_init();
     }
     if (warp == 8 && lane == 0) tma_prefetch_map(&map_k), tma_prefetch_map(&map_v);
-    attn_find_start<TC_THREADS, TC_ROWS, TC_KEYS, TC_ITEM>(a, &sh.start, sh.scan);
+    attn_find_start<TC_THREADS, ROWS, TC_KEYS, TC_ITEM>(a, &sh.start, sh.scan);
     if (sh.start.begin >= sh.start.end) {
         if (threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
         pdl_launch_dependents();
@@ -155,7 +158,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     tc_fence_after();
     const uint32_t tmem = sh.tmem_base;
     volatile int *abortp = &sh.abort_flag;
-    AttnWalk<TC_ROWS, TC_KEYS, TC_ITEM> w;
+    AttnWalk<ROWS, TC_KEYS, TC_ITEM> w;
     bool more = w.seek(a, sh.start), ok = true;
     if (!more && threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
 
@@ -167,7 +170,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const int behind = a.num_pages * a.kv_heads * a.page_size;  // first row behind the cache: zeros
         uint32_t nslot = 0, nkv = 0;
         while (more && ok) {
-            const TcItem t(a, w);
+            const TcItem<DPAD> t(a, w);
             const int32_t *table = a.block_table + (long long)w.request * a.max_pages;
             // lane b: row of the cache at which box b of a tile begins, and whether its page is missing
             auto look_up = [&](int n, bool &hole) -> int {
@@ -252,7 +255,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         };
         auto wait_slot = [&]() { return __all_sync(0xffffffffu, mbar_wait_abortable(&sh.kv_full[nslot % SLOTS], (nslot / SLOTS) & 1, abortp)); };
         while (more && ok) {
-            const TcItem im(a, w);
+            const TcItem<DPAD> im(a, w);
             const int lead = min(2, im.ntiles);
             if (t == 1 && im.rows <= 128) {  // nothing to multiply: this row tile's share of the slots is released in turn
 #pragma unroll 1
@@ -302,14 +305,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const int c = lane % CPR, r0 = lane / CPR, token_step = STEP / a.group, in_step = STEP - token_step * a.group;
         uint32_t use[2] = {0, 0};
         while (more && ok) {
-            const int item_rows = w.q.rows - w.tile * TC_ROWS;
+            const int item_rows = min(ROWS, w.q.rows - w.tile * ROWS);
             const T *q = static_cast<const T *>(a.q) + w.q.first * a.q_stride + (long long)w.head * a.group * a.head_dim + c * 8;
 #pragma unroll 1
             for (int t = 0; t < 2 && ok && item_rows > t * 128; ++t) {
                 if (use[t] > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait_abortable(&sh.q_empty[t], (use[t] - 1) & 1, abortp)))) break;
                 ++use[t];
                 unsigned char *dst = q_s + t * S::Q_BYTES + (c >> 3) * S::Q_PANEL;
-                int row = w.tile * TC_ROWS + t * 128 + r0, token = row / a.group, in = row - token * a.group;  // head of the group
+                int row = w.tile * ROWS + t * 128 + r0, token = row / a.group, in = row - token * a.group;  // head of the group
                 if (q_vec) {
 #pragma unroll 4
                     for (int r = r0; r < 128; r += STEP, row += STEP) {
@@ -349,14 +352,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         uint32_t nkv = 0, nslot = 0, g = 0, o_use = 0, pv_use = 0;  // key tiles and slots of the block so far; score tiles and items of the row tile
         // the next item that has rows for this tile
         auto take_item = [&]() {
-            while (more && t == 1 && w.q.rows - w.tile * TC_ROWS <= 128) {
+            while (more && t == 1 && min(ROWS, w.q.rows - w.tile * ROWS) <= 128) {
                 nkv += w.to - w.from, nslot += w.to - w.from + min(2, w.to - w.from);
                 more = w.next(a, sh.start);
             }
         };
         take_item();
         while (more && ok) {
-            const TcItem im(a, w);
+            const TcItem<DPAD> im(a, w);
             const int my_row = t * 128 + row_in;
             const bool have = my_row < im.rows, warp_has = t * 128 + (warp & 3) * 32 < im.rows;
             const int pos = have ? im.base + (im.row0 + my_row) / a.group : -1;
@@ -467,7 +470,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if (lane == 0) mbar_arrive(&sh.p_full[t][b]);
             }
             if (!ok) break;
-            const AttnWalk<TC_ROWS, TC_KEYS, TC_ITEM> done = w;
+            const AttnWalk<ROWS, TC_KEYS, TC_ITEM> done = w;
             const uint32_t nslot_done = nslot;  // the slots of the last products
             nslot += lead;
             more = w.next(a, sh.start);
@@ -506,7 +509,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     if (!whole) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) part[(c * 32 + i) * TC_ROWS] = __uint_as_float(o[i]);
+                        for (int i = 0; i < 32; ++i) part[(c * 32 + i) * ROWS] = __uint_as_float(o[i]);
                     } else if (have) {
                         T *d = dst + c * 32;
 #pragma unroll
@@ -519,7 +522,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         }
                     }
                 }
-                if (!whole) part[DPAD * TC_ROWS] = m, part[(DPAD + 1) * TC_ROWS] = l;
+                if (!whole) part[DPAD * ROWS] = m, part[(DPAD + 1) * ROWS] = l;
             }
             if (threadIdx.x == 0) {
                 if (!whole && done.from == 0)
@@ -540,24 +543,25 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_launch_dependents();
 }
 
-// The parts of a split tile lie column by column ([DPAD + 2][256], the last two the maximum and the sum): a warp's lanes
+// The parts of a split tile lie column by column ([DPAD + 2][ROWS], the last two the maximum and the sum): a warp's lanes
 // are 32 rows, its columns 16 of the head's.  Block (x, y): the item that block x of the main kernel began, rows 32 y ...
 template <class T, int DPAD>
 __global__ void __launch_bounds__(DPAD * 2) attn_tc_join_kernel(AttnArgs a) {
+    constexpr int ROWS = TcShape<DPAD>::ROWS;
     pdl_wait();
     const int4 item = a.joins[blockIdx.x];
     if (item.x < 0) return;
     const AttnRequest q = attn_request(a, item.x);
-    const int row = blockIdx.y * 32 + (threadIdx.x & 31), d0 = (threadIdx.x >> 5) * 16, rows = min(TC_ROWS, q.rows - item.z * TC_ROWS);
+    const int row = blockIdx.y * 32 + (threadIdx.x & 31), d0 = (threadIdx.x >> 5) * 16, rows = min(ROWS, q.rows - item.z * ROWS);
     if (row >= rows || d0 >= a.head_dim) return;
     const int parts = item.w - (int)blockIdx.x + 1;
     float m = -INFINITY, l = 0.0f, acc[16] = {};
     for (int i = 0; i < parts; ++i) {
         const float *p = a.parts + ((long long)(blockIdx.x + i) * 2 + (i == 0)) * TcShape<DPAD>::PART_FLOATS + row;
-        const float pm = p[DPAD * TC_ROWS], pl = p[(DPAD + 1) * TC_ROWS];
+        const float pm = p[DPAD * ROWS], pl = p[(DPAD + 1) * ROWS];
         float v[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) v[c] = p[(d0 + c) * TC_ROWS];
+        for (int c = 0; c < 16; ++c) v[c] = p[(d0 + c) * ROWS];
         if (pl == 0.0f) continue;  // a part that saw nothing
         const float top = fmaxf(m, pm), w0 = exp2f(m - top), w1 = exp2f(pm - top);
         l = l * w0 + pl * w1, m = top;
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(DPAD * 2) attn_tc_join_kernel(AttnArgs a) {
         for (int c = 0; c < 16; ++c) acc[c] = acc[c] * w0 + v[c] * w1;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int at = item.z * TC_ROWS + row, token = at / a.group, head = item.y * a.group + at % a.group;
+    const int at = item.z * ROWS + row, token = at / a.group, head = item.y * a.group + at % a.group;
     T *dst = static_cast<T *>(a.out) + (q.first + token) * a.out_stride + (long long)head * a.head_dim + d0;
     const uintptr_t phase = (uintptr_t)dst;
 #pragma unroll
@@ -612,13 +616,13 @@ static int attn_tc_launch_dim(AttnArgs a, bool bf16, int longest_rows, void *wor
     const uint32_t idesc_qk = common | ((TC_KEYS >> 3) << 17), idesc_pv = common | (1u << 16) | ((DPAD >> 3) << 17);
     st = launch_kernel(attn_tc_kernel<T, DPAD>, dim3(grid), dim3(TC_THREADS), S::SMEM, s, false, map_k, map_v, a, idesc_qk, idesc_pv);
     if (st) return st;
-    return launch_kernel(attn_tc_join_kernel<T, DPAD>, dim3(grid, min((longest_rows + 31) / 32, TC_ROWS / 32)), dim3(DPAD * 2), 0, s, true, a);
+    return launch_kernel(attn_tc_join_kernel<T, DPAD>, dim3(grid, min((longest_rows + 31) / 32, S::ROWS / 32)), dim3(DPAD * 2), 0, s, true, a);
 }
 
-// Shapes the kernel takes: heads of up to 128, pages of a power of two of keys from 8 on (a box of 8 rows is the
+// Shapes the kernel takes: heads of up to 256, pages of a power of two of keys from 8 on (a box of 8 rows is the
 // swizzle's period), 16-byte aligned caches whose rows a 32-bit coordinate counts.
 bool attn_tc_eligible(const AttnArgs &a) {
-    return a.head_dim <= 128 && a.page_shift >= 3 && a.num_pages > 0 && aligned_to(a.k_cache, 16) && aligned_to(a.v_cache, 16) &&
+    return a.head_dim <= 256 && a.page_shift >= 3 && a.num_pages > 0 && aligned_to(a.k_cache, 16) && aligned_to(a.v_cache, 16) &&
            (long long)a.num_pages * a.kv_heads * a.page_size < (1LL << 31) - 1024 && encode_tiled_fn();
 }
 
@@ -626,9 +630,11 @@ int attn_tc_launch(const AttnArgs &a, int type, int longest_rows, void *workspac
     const bool bf16 = type == TB200_TYPE_BF16;
     if (a.head_dim <= 64)
         return bf16 ? attn_tc_launch_dim<__nv_bfloat16, 64>(a, true, longest_rows, workspace, di, s) : attn_tc_launch_dim<__half, 64>(a, false, longest_rows, workspace, di, s);
-    return bf16 ? attn_tc_launch_dim<__nv_bfloat16, 128>(a, true, longest_rows, workspace, di, s) : attn_tc_launch_dim<__half, 128>(a, false, longest_rows, workspace, di, s);
+    if (a.head_dim <= 128)
+        return bf16 ? attn_tc_launch_dim<__nv_bfloat16, 128>(a, true, longest_rows, workspace, di, s) : attn_tc_launch_dim<__half, 128>(a, false, longest_rows, workspace, di, s);
+    return bf16 ? attn_tc_launch_dim<__nv_bfloat16, 256>(a, true, longest_rows, workspace, di, s) : attn_tc_launch_dim<__half, 256>(a, false, longest_rows, workspace, di, s);
 }
 
-size_t attn_tc_workspace(int head_dim) { return head_dim <= 64 ? TcShape<64>::WORKSPACE : head_dim <= 128 ? TcShape<128>::WORKSPACE : 0; }
+size_t attn_tc_workspace(int head_dim) { return head_dim <= 64 ? TcShape<64>::WORKSPACE : head_dim <= 128 ? TcShape<128>::WORKSPACE : TcShape<256>::WORKSPACE; }
 
 }  // namespace tb200
