@@ -61,7 +61,8 @@ template <int DPAD, bool SPLIT_KEYS>
 struct AtShape {
     static constexpr int ROWS = SPLIT_KEYS ? 16 : 64;
     // The copies in flight hide the memory's latency, several blocks an SM each other's arithmetic: with 128 columns three
-    // blocks of two stages read 64 requests of up to 8192 keys in 196 us, two of three in 230 us or more; with 64 columns
+    // blocks of two stages read 64 requests of up to 8192 keys in 242 us where two of three took 302 us (196 us since the
+    // copies' addresses cost less); with 64 columns
     // four blocks of three stages in 113 us, three of four in 127 us.
     static constexpr int STAGES = DPAD == 64 ? (SPLIT_KEYS ? 3 : 4) : DPAD == 128 ? 2 : SPLIT_KEYS ? 3 : 2;
     static constexpr int BLOCKS_PER_SM = DPAD == 256 ? 1 : !SPLIT_KEYS ? 2 : DPAD == 64 ? 4 : 3;
