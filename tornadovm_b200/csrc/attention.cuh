@@ -218,7 +218,8 @@ struct AttnWalk {
             if (++head >= a.kv_heads) {
                 head = 0;
                 do {
-                    q = attn_request(a, ++request);
+                    if (++request >= a.requests) return false;  // lengths that changed meanwhile must not lead past the arrays
+                    q = attn_request(a, request);
                 } while (q.rows == 0);
             }
         }
