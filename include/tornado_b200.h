@@ -427,7 +427,7 @@ enum tb200_quant_format { TB200_Q_INT8 = 0, TB200_Q_E4M3 = 1, TB200_Q_E5M2 = 2 }
  *   scale = max |y| / 127, 448 or 57344 of the group, 1 for a group of zeros;
  *   int8: floor(y / scale + 1/2), the rule of tb200_quantize_x; fp8: to the nearest, ties to even.
  * A group that holds an infinity or a NaN gets that as its scale and zeros as its values, so that the values it stands
- * for are NaN. */
+ * for are NaN.  cols <= 2^30. */
 int tb200_rmsnorm_quant(int rows, int cols, int type, const void *x, long long x_stride, const void *residual, void *residual_out,
                         const float *weight, float eps, int format, int group, uint8_t *q, float *scales, tb200_stream_t stream);
 

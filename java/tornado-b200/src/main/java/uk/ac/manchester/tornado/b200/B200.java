@@ -234,7 +234,7 @@ public final class B200 {
     }
 
     private static void checkNorm(String name, int rows, int cols, TornadoNativeArray x, FloatArray weight, float eps, int format, int group, TornadoNativeArray q, FloatArray scales) {
-        check(rows >= 0 && cols >= 1, "B200 " + name + " requires rows >= 0 and cols >= 1; got rows=" + rows + ", cols=" + cols);
+        check(rows >= 0 && cols >= 1 && cols <= 1 << 30, "B200 " + name + " requires rows >= 0 and 1 <= cols <= 2^30; got rows=" + rows + ", cols=" + cols);
         check(format >= QUANT_INT8 && format <= QUANT_E5M2, "B200 " + name + " knows the formats 0 (int8), 1 (e4m3), 2 (e5m2); got " + format);
         check(group == 0 || group == 32 || group == 64 || group == 128, "B200 " + name + " requires groups of 32, 64 or 128 columns, or 0 for a scale per row; got " + group);
         check(eps >= 0.0f && eps <= Float.MAX_VALUE, "B200 " + name + " requires a finite eps >= 0; got " + eps);

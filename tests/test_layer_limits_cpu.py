@@ -1,0 +1,21 @@
+"""Calls of the decoder-layer operators that lie beyond what their index arithmetic takes: refused on the host, before
+anything is launched (no GPU needed)."""
+import pytest
+
+from test_layer_cpu import INVALID, P, norm
+
+
+@pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) - 8192, (1 << 31) - 1])
+def test_norm_refuses_rows_that_32_bits_do_not_index(lib, cols):
+    """A thread's next column, c + 8192, would pass 2**31 - 1 and come back negative."""
+    for kw in (dict(group=0), dict(group=32), dict(type=0), dict(x=P + 4, type=0)):
+        assert norm(lib, cols=cols, x_stride=1 << 31, **kw) == INVALID
+
+
+def test_factories_refuse_what_the_library_refuses():
+    """The arrays are checked behind the sizes, so that none of that size is needed."""
+    from tornadovm_b200.arrays import FloatArray, Int8Array
+    from tornadovm_b200.b200 import B200
+    f = FloatArray
+    with pytest.raises(RuntimeError, match="cols <= 2"):
+        B200.rmsnormQuant(1, (1 << 30) + 1, f(4), f(4), 1e-5, "int8", 32, Int8Array(4), f(4))

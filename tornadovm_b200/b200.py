@@ -233,7 +233,7 @@ class B200:
 
     @staticmethod
     def _norm(name, rows, cols, x, residual, weight, eps, fmt, group, q, scales):
-        _check(rows >= 0 and cols >= 1, f"B200 {name} requires rows >= 0 and cols >= 1; got rows={rows}, cols={cols}")
+        _check(rows >= 0 and 1 <= cols <= 1 << 30, f"B200 {name} requires rows >= 0 and 1 <= cols <= 2^30; got rows={rows}, cols={cols}")
         _check(fmt in QUANT_FORMATS, f"B200 {name} knows the formats {', '.join(QUANT_FORMATS)}; got {fmt}")
         _check(group in (0, 32, 64, 128), f"B200 {name} requires groups of 32, 64 or 128 columns, or 0 for a scale per row; got {group}")
         _check(0.0 <= eps < float("inf"), f"B200 {name} requires a finite eps >= 0; got {eps}")

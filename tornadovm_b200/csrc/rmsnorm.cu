@@ -361,7 +361,8 @@ using namespace tb200;
 
 extern "C" int tb200_rmsnorm_quant(int rows, int cols, int type, const void *x, long long x_stride, const void *residual, void *residual_out,
                                    const float *weight, float eps, int format, int group, uint8_t *q, float *scales, tb200_stream_t stream) {
-    if (rows < 0 || cols < 1 || !valid_type(type) || x_stride < cols) return TB200_ERR_INVALID_ARG;
+    // a thread's next column, up to 8192 behind the last one, is still a 32-bit number
+    if (rows < 0 || cols < 1 || cols > (1 << 30) || !valid_type(type) || x_stride < cols) return TB200_ERR_INVALID_ARG;
     if (format < TB200_Q_INT8 || format > TB200_Q_E5M2 || !(group == 0 || group == 32 || group == 64 || group == 128)) return TB200_ERR_INVALID_ARG;
     if (!(eps >= 0.0f) || eps > 3.402823466e38f) return TB200_ERR_INVALID_ARG;
     if (rows == 0) return TB200_OK;
