@@ -480,7 +480,7 @@ int tb200_rope_append(int tokens, int q_heads, int kv_heads, int head_dim, int i
  * max_new: an upper bound on the rows of one request (0: unknown); it only chooses kernels and never changes what is
  * computed.  The context of a request is split over the GPU and joined in a fixed order, so equal calls give equal
  * results.  The workspace (16-byte aligned; tb200_paged_attention_workspace_bytes) needs no initialisation; two calls
- * that can run at the same time need one each.  max_pages * page_size <= 2^30. */
+ * that can run at the same time need one each.  requests, tokens * q_heads / kv_heads and max_pages * page_size <= 2^30. */
 size_t tb200_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim);
 int tb200_paged_attention(int tokens, int requests, int max_new, int q_heads, int kv_heads, int head_dim, int type, const void *q,
                           long long q_stride, const int32_t *cu_new, const int32_t *kv_lens, const int32_t *block_table, int max_pages,

@@ -293,7 +293,7 @@ public final class B200 {
     public static LibraryTaskDescriptor pagedAttention(int tokens, int requests, int maxNew, int qHeads, int kvHeads, int headDim, TornadoNativeArray q, IntArray cuNew, IntArray kvLens,
             IntArray blockTable, int pageSize, TornadoNativeArray kCache, TornadoNativeArray vCache, float scale, int window, TornadoNativeArray out) {
         int pages = cachePages("pagedAttention", kvHeads, headDim, pageSize, kCache, vCache);
-        check(tokens >= 0 && requests >= 1 && maxNew >= 0 && window >= 0, "B200 pagedAttention requires tokens, maxNew, window >= 0 and requests >= 1");
+        check(tokens >= 0 && requests >= 1 && requests <= 1 << 30 && maxNew >= 0 && window >= 0, "B200 pagedAttention requires tokens, maxNew, window >= 0 and 1 <= requests <= 2^30");
         check(qHeads >= kvHeads && qHeads % kvHeads == 0, "B200 pagedAttention requires qHeads to be a multiple of kvHeads; got " + qHeads + ", " + kvHeads);
         check(headDim % 8 == 0 && headDim <= 256, "B200 pagedAttention requires headDim to be a multiple of 8 up to 256; got " + headDim);
         check(scale > 0.0f && scale <= Float.MAX_VALUE, "B200 pagedAttention requires a finite scale > 0; got " + scale);

@@ -2,7 +2,7 @@
 anything is launched (no GPU needed)."""
 import pytest
 
-from test_layer_cpu import INVALID, P, norm
+from test_layer_cpu import INVALID, P, attention, norm
 
 
 @pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) - 8192, (1 << 31) - 1])
@@ -12,10 +12,19 @@ def test_norm_refuses_rows_that_32_bits_do_not_index(lib, cols):
         assert norm(lib, cols=cols, x_stride=1 << 31, **kw) == INVALID
 
 
+def test_attention_refuses_requests_that_32_bits_do_not_index(lib):
+    for requests in ((1 << 30) + 1, (1 << 31) - 1):
+        assert attention(lib, requests=requests) == INVALID
+        assert lib.tb200_paged_attention_workspace_bytes(3, requests, 4, 2, 64) == 0
+
+
 def test_factories_refuse_what_the_library_refuses():
     """The arrays are checked behind the sizes, so that none of that size is needed."""
-    from tornadovm_b200.arrays import FloatArray, Int8Array
+    from tornadovm_b200.arrays import FloatArray, HalfFloatArray, Int8Array, IntArray
     from tornadovm_b200.b200 import B200
-    f = FloatArray
+    f, h = FloatArray, HalfFloatArray
     with pytest.raises(RuntimeError, match="cols <= 2"):
         B200.rmsnormQuant(1, (1 << 30) + 1, f(4), f(4), 1e-5, "int8", 32, Int8Array(4), f(4))
+    k = h(2 * 16 * 64)
+    with pytest.raises(RuntimeError, match="requests <= 2"):
+        B200.pagedAttention(1, (1 << 30) + 1, 0, 4, 2, 64, h(256), IntArray(2), IntArray(1), IntArray(1), 16, k, k, 0.1, 0, h(256))

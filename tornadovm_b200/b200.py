@@ -306,7 +306,7 @@ class B200:
         """Causal attention of each request's new tokens over its pages of the cache, the new tokens included
         (tb200_paged_attention); ``window`` 0: no limit, ``maxNew`` 0: no bound known."""
         kind, pages = B200._cache("pagedAttention", kvHeads, headDim, pageSize, kCache, vCache)
-        _check(tokens >= 0 and requests >= 1 and maxNew >= 0 and window >= 0, "B200 pagedAttention requires tokens, maxNew, window >= 0 and requests >= 1")
+        _check(tokens >= 0 and 1 <= requests <= 1 << 30 and maxNew >= 0 and window >= 0, "B200 pagedAttention requires tokens, maxNew, window >= 0 and 1 <= requests <= 2^30")
         _check(qHeads >= kvHeads and qHeads % kvHeads == 0, f"B200 pagedAttention requires qHeads to be a multiple of kvHeads; got {qHeads}, {kvHeads}")
         _check(headDim % 8 == 0 and headDim <= 256, f"B200 pagedAttention requires headDim to be a multiple of 8 up to 256; got {headDim}")
         _check(0.0 < scale < float("inf"), f"B200 pagedAttention requires a finite scale > 0; got {scale}")

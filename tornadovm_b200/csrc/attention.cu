@@ -471,7 +471,7 @@ size_t attn_any_workspace(int head_dim) {
 using namespace tb200;
 
 static bool attn_shape_ok(int tokens, int requests, int q_heads, int kv_heads, int head_dim) {
-    return tokens >= 0 && requests >= 0 && kv_heads >= 1 && q_heads >= kv_heads && q_heads % kv_heads == 0 && head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0 &&
+    return tokens >= 0 && requests >= 0 && requests <= (1 << 30) && kv_heads >= 1 && q_heads >= kv_heads && q_heads % kv_heads == 0 && head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0 &&
            (long long)tokens * (q_heads / kv_heads) <= (1LL << 30) && q_heads <= 65536;
 }
 
