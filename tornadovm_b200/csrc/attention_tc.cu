@@ -544,7 +544,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 }
 
 // The parts of a split tile lie column by column ([DPAD + 2][ROWS], the last two the maximum and the sum): a warp's lanes
-// are 32 rows, its columns 16 of the head's.  Block (x, y): the item that block x of the main kernel began, rows 32 y ...
+// are 32 rows, its columns 16 of the head's.  Block (x, y): the item that block x of the main kernel began, every gridDim.y-th
+// 32 rows of it from 32 y on.
 template <class T, int DPAD>
 __global__ void __launch_bounds__(DPAD * 2) attn_tc_join_kernel(AttnArgs a) {
     constexpr int ROWS = TcShape<DPAD>::ROWS;
@@ -552,33 +553,35 @@ __global__ void __launch_bounds__(DPAD * 2) attn_tc_join_kernel(AttnArgs a) {
     const int4 item = a.joins[blockIdx.x];
     if (item.x < 0) return;
     const AttnRequest q = attn_request(a, item.x);
-    const int row = blockIdx.y * 32 + (threadIdx.x & 31), d0 = (threadIdx.x >> 5) * 16, rows = min(ROWS, q.rows - item.z * ROWS);
-    if (row >= rows || d0 >= a.head_dim) return;
-    const int parts = item.w - (int)blockIdx.x + 1;
-    float m = -INFINITY, l = 0.0f, acc[16] = {};
-    for (int i = 0; i < parts; ++i) {
-        const float *p = a.parts + ((long long)(blockIdx.x + i) * 2 + (i == 0)) * TcShape<DPAD>::PART_FLOATS + row;
-        const float pm = p[DPAD * ROWS], pl = p[(DPAD + 1) * ROWS];
-        float v[16];
+    const int d0 = (threadIdx.x >> 5) * 16, rows = min(ROWS, q.rows - item.z * ROWS), parts = item.w - (int)blockIdx.x + 1;
+    if (d0 >= a.head_dim) return;
+    // gridDim.y follows a hint, the rows do not
+    for (int row = blockIdx.y * 32 + (threadIdx.x & 31); row < rows; row += gridDim.y * 32) {
+        float m = -INFINITY, l = 0.0f, acc[16] = {};
+        for (int i = 0; i < parts; ++i) {
+            const float *p = a.parts + ((long long)(blockIdx.x + i) * 2 + (i == 0)) * TcShape<DPAD>::PART_FLOATS + row;
+            const float pm = p[DPAD * ROWS], pl = p[(DPAD + 1) * ROWS];
+            float v[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) v[c] = p[(d0 + c) * ROWS];
-        if (pl == 0.0f) continue;  // a part that saw nothing
-        const float top = fmaxf(m, pm), w0 = exp2f(m - top), w1 = exp2f(pm - top);
-        l = l * w0 + pl * w1, m = top;
+            for (int c = 0; c < 16; ++c) v[c] = p[(d0 + c) * ROWS];
+            if (pl == 0.0f) continue;  // a part that saw nothing
+            const float top = fmaxf(m, pm), w0 = exp2f(m - top), w1 = exp2f(pm - top);
+            l = l * w0 + pl * w1, m = top;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) acc[c] = acc[c] * w0 + v[c] * w1;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int at = item.z * ROWS + row, token = at / a.group, head = item.y * a.group + at % a.group;
-    T *dst = static_cast<T *>(a.out) + (q.first + token) * a.out_stride + (long long)head * a.head_dim + d0;
-    const uintptr_t phase = (uintptr_t)dst;
+            for (int c = 0; c < 16; ++c) acc[c] = acc[c] * w0 + v[c] * w1;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int at = item.z * ROWS + row, token = at / a.group, head = item.y * a.group + at % a.group;
+        T *dst = static_cast<T *>(a.out) + (q.first + token) * a.out_stride + (long long)head * a.head_dim + d0;
+        const uintptr_t phase = (uintptr_t)dst;
 #pragma unroll
-    for (int c = 0; c < 16; c += 8) {  // whole sectors where the alignment allows it
-        if (d0 + c >= a.head_dim) break;
-        uint32_t h[4];
+        for (int c = 0; c < 16; c += 8) {  // whole sectors where the alignment allows it
+            if (d0 + c >= a.head_dim) break;
+            uint32_t h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = pack2(acc[c + 2 * i] * inv, acc[c + 2 * i + 1] * inv, T());
-        tc_store8(dst + c, h, phase);
+            for (int i = 0; i < 4; ++i) h[i] = pack2(acc[c + 2 * i] * inv, acc[c + 2 * i + 1] * inv, T());
+            tc_store8(dst + c, h, phase);
+        }
     }
 }
 
