@@ -470,7 +470,7 @@ int tb200_rope_append(int tokens, int q_heads, int kv_heads, int head_dim, int i
  * cu_new[r + 1] - 1 (ascending; rows at or above `tokens` are not touched), query head h reads kv head
  * h / (q_heads / kv_heads), and row i stands at position p = kv_lens[r] - rows of r + i.  Key j of the request lies in
  * page block_table[r][j / page_size] (rows of max_pages entries) and is visible when 0 <= j <= p, j > p - window
- * (window 0: no limit), j < max_pages * page_size, and its page is one of the cache's num_pages (others, -1 among
+ * (window 0, or 2^30 and more: no limit), j < max_pages * page_size, and its page is one of the cache's num_pages (others, -1 among
  * them, count as masked).  A row that sees no key, or only scores of -infinity, gives zeros.  What the cache holds at
  * places that a row does not see never reaches it, infinities and NaN included.
  * q, out and the caches [num_pages][kv_heads][page_size][head_dim] are of one type, F16 or BF16; head_dim is a multiple

@@ -18,3 +18,15 @@ def test_attention_stores_every_row_whatever_the_bound_on_new_tokens_says(lib, d
     p = Paged(rng, [2000], [90], heads, kv_heads, dim, 16, BF16, pad=2)
     check_attention(lib, p, max_new=max_new)
     check_attention(lib, p, max_new=90)
+
+
+# ---- attention: windows that end nowhere --------------------------------------------------------------------------------
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 3, 2 ** 30 + 1, 2 ** 30])
+@pytest.mark.parametrize("new,header", [(10, 16), (40, 16), (40, 24)])
+def test_attention_window_without_an_end(lib, window, new, header):
+    """kv_len below the new tokens, so that the first rows stand in front of key 0: none of the others loses its keys."""
+    rng = np.random.default_rng(new)
+    p = Paged(rng, [0, 70], [new, new], 4, 4, 64, 16, F16)
+    p.kv[0] = new - 5
+    a = check_attention(lib, p, window, header=header)
+    assert np.array_equal(a, run_attention(lib, p, 0, header=header))

@@ -503,7 +503,8 @@ extern "C" int tb200_paged_attention(int tokens, int requests, int max_new, int 
     a.q = q, a.k_cache = k_cache, a.v_cache = v_cache, a.cu_new = cu_new, a.kv_lens = kv_lens, a.block_table = block_table, a.out = out;
     a.q_stride = q_stride, a.out_stride = out_stride, a.scale_log2 = scale * 1.4426950408889634f;
     a.tokens = tokens, a.requests = requests, a.q_heads = q_heads, a.kv_heads = kv_heads, a.group = q_heads / kv_heads, a.head_dim = head_dim;
-    a.max_pages = max_pages, a.page_size = page_size, a.num_pages = num_pages, a.window = window;
+    a.max_pages = max_pages, a.page_size = page_size, a.num_pages = num_pages;
+    a.window = window < (1 << 30) ? window : 0;  // positions are below 2^30: a wider window limits nothing, and a position minus a window stays a 32-bit number
     a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
     const long long longest = (long long)(max_new > 0 ? min(max_new, tokens) : tokens) * a.group;
     const int rows = (int)min(longest, 0x7FFFFFFFLL);
