@@ -30,3 +30,59 @@ def test_attention_window_without_an_end(lib, window, new, header):
     p.kv[0] = new - 5
     a = check_attention(lib, p, window, header=header)
     assert np.array_equal(a, run_attention(lib, p, 0, header=header))
+
+
+# ---- norm: values near the ends of fp32 ---------------------------------------------------------------------------------
+def check_far_norm(lib, x, weight, kind, fmt, group, eps, residual=None, **kw):
+    """Codes and scales against 64 bits.  As for values near 1: the sum of `cols` squares, the root, products and
+    quotients move y by `rel` of itself.  Beside that h * weight is rounded to half of the smallest subnormal at worst,
+    2**-150, which the norm's factor multiplies; a factor above 2**15 meets no such products (values of rows that small
+    are taken nearer to 1 first)."""
+    q, scales, stored = run_norm(lib, x, residual, weight, kind, fmt, group, eps=eps, **kw)
+    rx, rr = from_bits(to_bits(x, kind), kind), None if residual is None else from_bits(to_bits(residual, kind), kind)
+    w32 = weight.astype(np.float32)
+    ratio, want, h = ol.rmsnorm_quant(rx, rr, w32, float(np.float32(eps)), fmt, group)
+    cols = x.shape[1]
+    rel = (0.5 * cols + 12) * 2.0 ** -24
+    with np.errstate(all="ignore"):
+        factor = 1 / np.sqrt((h * h).mean(1) + float(np.float32(eps)))
+    lost = np.minimum(factor, 2.0 ** 15)[:, None] * 2.0 ** -150
+    assert np.isfinite(want).all()
+    assert np.all(np.abs(scales - want) <= rel * want + lost + 2.0 ** -149)
+    g = group or cols
+    scale_of = np.repeat(want, g, 1)[:, :cols]
+    val = q.view(np.int8).astype(np.float64) if fmt == "int8" else fp8_values(q, fmt)
+    assert np.isfinite(val).all()
+    moved = np.abs(ratio) * (2 * rel + 2.0 ** -23) + lost / scale_of
+    if fmt == "int8":
+        bound = 0.5 + moved + 2.0 ** -17
+    else:
+        m, low = (3, -9) if fmt == "e4m3" else (2, -16)
+        _, e = np.frexp(np.maximum(np.abs(ratio) + moved, 1e-300))
+        bound = 0.5 * np.exp2(np.maximum(e - 1 - m, low).astype(np.float64)) + moved
+    off = np.abs(val - ratio)
+    assert np.all(off <= bound), (off - bound).max()
+    if stored is not None:
+        s = from_bits(stored, kind)
+        assert np.all(np.abs(s - h) <= (HALF_STEP[kind] + 2.0 ** -24) * np.abs(h) + HALF_TINY[kind])
+    return q, scales
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("fmt,group", [("int8", 32), ("int8", 0), ("e4m3", 128), ("e4m3", 0), ("e5m2", 64), ("e5m2", 32)])
+@pytest.mark.parametrize("rows,cols", [(9, 256), (400, 512), (9, 33024)])
+def test_norm_groups_down_to_subnormals(lib, kind, fmt, group, rows, cols):
+    """Dead groups in an ordinary row, and rows that are tiny altogether (the factor of the norm is 316 there), with zeros
+    among them: no code is a NaN, and none is off."""
+    rng = np.random.default_rng(cols)
+    w = 1 + 0.3 * rng.standard_normal(cols)
+    x = rng.standard_normal((rows, cols))
+    for i, tiny in enumerate((1e-30, 1e-34, 1e-36, 1e-37, 1e-38, 1e-39, 1e-41, 0.0)):
+        x[i] *= 0.01
+        x[i, 128:256] *= tiny * 100
+        x[i, 130:140] = 0
+    check_far_norm(lib, x, w, kind, fmt, group, 1e-5)
+    for i, tiny in enumerate((1e-20, 1e-30, 1e-34, 1e-36, 1e-37, 1e-38, 1e-39, 1e-41)):
+        x[i] = rng.standard_normal(cols) * tiny
+        x[i, 3:200:7] = 0
+    check_far_norm(lib, x, w, kind, fmt, group, 1e-5)

@@ -50,7 +50,17 @@ __device__ __forceinline__ float group_scale(float top_y, int format, float &inv
     return finite ? scale : top_y;
 }
 
-// Eight values of h * weight, times the norm's factor over the scale, as eight bytes; inv 0: a group that is not finite.
+// What turns eight values of h * weight into codes: the norm's factor over the scale, rounded once.  Where that product is
+// beyond fp32 (the largest |h * weight| of the group is below top / 3.4e38, its y is not) the values become y first.
+__device__ __forceinline__ float code_factor(float (&h)[8], float inv, float rstd) {
+    const float factor = inv * rstd;
+    if (factor <= 3.402823466e38f) return factor;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] *= rstd;
+    return inv;
+}
+
+// Eight values of h * weight, times `factor`, as eight bytes; inv 0: a group that is not finite.
 __device__ __forceinline__ uint2 to_8bit(const float (&y)[8], float inv, float factor, int format) {
     if (inv == 0.0f) return make_uint2(0, 0);
     uint32_t w[2];
@@ -265,7 +275,10 @@ __global__ void __launch_bounds__(NV <= 2 && STAGES == 0 ? 1024 : 512) rmsnorm_k
                 const float scale = group_scale(group_max(part[i], a.group) * rstd, a.format, inv);
                 if (c < a.cols && (c & (a.group - 1)) == 0) a.scales[row * a.groups + (c >> a.group_shift)] = scale;
             }
-            if (c < a.cols) store_q<ALIGN>(a, row, c, h[i], inv, inv * rstd);
+            if (c < a.cols) {
+                const float factor = code_factor(h[i], inv, rstd);
+                store_q<ALIGN>(a, row, c, h[i], inv, factor);
+            }
         }
     }
 }
@@ -308,7 +321,10 @@ __global__ void __launch_bounds__(1024) rmsnorm_long_kernel(NormArgs a) {
                 const float scale = group_scale(group_max(largest(h), a.group) * rstd, a.format, inv);
                 if (c < a.cols && (c & (a.group - 1)) == 0) a.scales[row * a.groups + (c >> a.group_shift)] = scale;
             }
-            if (c < a.cols) store_q<ALIGN>(a, row, c, h, inv, inv * rstd);
+            if (c < a.cols) {
+                const float factor = code_factor(h, inv, rstd);
+                store_q<ALIGN>(a, row, c, h, inv, factor);
+            }
         }
     }
 }
