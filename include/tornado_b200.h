@@ -422,7 +422,7 @@ enum tb200_quant_format { TB200_Q_INT8 = 0, TB200_Q_E4M3 = 1, TB200_Q_E5M2 = 2 }
  * x [rows] rows of `cols` elements of `type`, x_stride elements apart (>= cols); residual and residual_out [rows][cols]
  * of the same type, each may be NULL (nothing is added / stored), and residual_out may be residual, or x when
  * x_stride == cols; weight [cols] fp32.  The sum, the norm and the quantisation are fp32: y is that of the sum before
- * residual_out's rounding.  q [rows][cols] holds int8, e4m3 or e5m2 (format) with one fp32 scale per `group` columns
+ * residual_out's rounding, at any magnitude of h that fp32 holds (weights up to 2^32).  q [rows][cols] holds int8, e4m3 or e5m2 (format) with one fp32 scale per `group` columns
  * (32, 64, 128; the last group of a row may be shorter) in scales [rows][ceil(cols / group)], or one per row (group 0).
  *   scale = max |y| / 127, 448 or 57344 of the group, 1 for a group of zeros;
  *   int8: floor(y / scale + 1/2), the rule of tb200_quantize_x; fp8: to the nearest, ties to even.

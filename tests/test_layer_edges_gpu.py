@@ -86,3 +86,53 @@ def test_norm_groups_down_to_subnormals(lib, kind, fmt, group, rows, cols):
         x[i] = rng.standard_normal(cols) * tiny
         x[i, 3:200:7] = 0
     check_far_norm(lib, x, w, kind, fmt, group, 1e-5)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("fmt,group", [("int8", 32), ("e4m3", 0), ("e5m2", 128)])
+@pytest.mark.parametrize("rows,cols", [(12, 96), (12, 4096), (500, 512), (12, 8200), (12, 16400), (320, 16400), (12, 33024), (12, 33001)])
+@pytest.mark.parametrize("eps", [0.0, 1e-35, 1e-5])
+def test_norm_of_rows_whose_squares_leave_fp32(lib, kind, fmt, group, rows, cols, eps):
+    """The norm does not depend on a row's magnitude, so long as the sum h and the products h * weight are finite."""
+    rng = np.random.default_rng(cols + int(eps * 1e6))
+    w = 1 + 0.3 * rng.standard_normal(cols)
+    x = rng.standard_normal((rows, cols))
+    for i, size in enumerate((1e18, 1e25, 3e37, 1e-15, 1e-21, 1e-30, 1e-37, 1e-40)):
+        x[i] *= size
+    x[8, :40] *= 1e30            # huge values beside ordinary ones
+    x[9, 50] = 3e38              # one huge value alone
+    x[9, 0:32] *= 1e-3
+    x[10, 20:96] *= 1e-25        # tiny groups in an ordinary row
+    x[11, 1] = 1e21              # a huge channel that the weights leave out, for the row with it
+    check_far_norm(lib, x, w, kind, fmt, group, eps, residual=np.zeros_like(x), place="residual")
+    w[1] = 0
+    check_far_norm(lib, x[11:12], w, kind, fmt, group, eps)
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("place", ["own", "residual", "x", "none"])
+@pytest.mark.parametrize("rows,cols", [(12, 512), (500, 512), (12, 9000), (400, 18000), (12, 33000), (400, 61)])
+@pytest.mark.parametrize("header", [16, 24])
+def test_norm_of_far_rows_wherever_the_sum_goes(lib, kind, place, rows, cols, header):
+    """Rows far from 1 are read again when the others are done: the sum may stand in their inputs' place by then."""
+    rng = np.random.default_rng(cols + header)
+    x, r, w = rng.standard_normal((rows, cols)), rng.standard_normal((rows, cols)), 1 + 0.3 * rng.standard_normal(cols)
+    far = np.arange(rows) % 5 == 1
+    size = 1e3 if kind == F16 else 1e25
+    x[far] *= size
+    r[far] *= size * 0.01
+    r[np.arange(rows) % 5 == 3] *= 1e-3 if kind == F16 else 1e-30
+    x[np.arange(rows) % 5 == 3] *= 1e-3 if kind == F16 else 1e-30
+    check_far_norm(lib, x, w, kind, "int8", 32, 0.0, residual=r, place=place, header=header)
+    check_far_norm(lib, x, w, kind, "e4m3", 0, 1e-5, residual=r, place=place, header=header)
+
+
+@pytest.mark.parametrize("kind,place", [(BF16, "residual"), (BF16, "own"), (F32, "x")])
+def test_norm_of_far_rows_among_more_rows_than_a_block_remembers(lib, kind, place):
+    rng = np.random.default_rng(11)
+    rows, cols = 148 * 28 * 32 + 8001, 64
+    x, r, w = rng.standard_normal((rows, cols), np.float32), rng.standard_normal((rows, cols), np.float32), 1 + 0.3 * rng.standard_normal(cols)
+    far = rng.random(rows) < 0.01
+    far[[0, rows - 1]] = True
+    x[far] *= 1e25
+    check_far_norm(lib, x.astype(np.float64), w, kind, "int8", 32, 1e-5, residual=r.astype(np.float64), place=place)

@@ -14,10 +14,12 @@
 // the 4, 8 or 16 lanes that hold it.  Rows that outgrow the registers (above 32768 columns) are read again instead.
 //
 // A thread holds eight consecutive columns per 16-byte load.  Few rows are a matter of latency: a thread for each eight
-// columns.  Many rows are one of instructions and of bytes in flight: a thread for 16 columns, and the next two rows of a
-// block on their way to shared memory while it works on one (8192 x 4096 bf16 to e4m3: 47 us, 75 us with a thread for
-// each eight columns and no rows ahead).
+// columns.  Many rows are one of instructions and of bytes in flight: a thread for 16 columns, its weights in registers, and
+// the next two rows of a block on their way to shared memory while it works on one (8192 x 4096 bf16 to e4m3: 42 us, 47 us
+// with the weights read for each row, 75 us with a thread for each eight columns and no rows ahead).
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 #define TB200_OP_CLASS TB200_PREPARE_LAYER
 #include "layer_common.cuh"
@@ -122,6 +124,18 @@ __device__ __forceinline__ void load_sum(const NormArgs &a, long long row, int c
     }
 }
 
+// Columns c .. c + 7 of a row of an fp32 residual_out.
+template <int ALIGN>
+__device__ __forceinline__ void load_stored(const NormArgs &a, long long row, int c, float (&h)[8]) {
+    const float *p = static_cast<const float *>(a.residual_out) + row * a.cols + c;
+    if constexpr (ALIGN != 0) {
+        load8<ALIGN>(p, h);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = c + j < a.cols ? p[j] : 0.0f;
+    }
+}
+
 template <int ALIGN>
 __device__ __forceinline__ void load_weight(const NormArgs &a, int c, float (&w)[8]) {
     if constexpr (ALIGN != 0) {
@@ -142,6 +156,22 @@ __device__ __forceinline__ void store_sum(const NormArgs &a, long long row, int 
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (c + j < a.cols) from_f32(p[j], h[j]);
+    }
+}
+
+// the same from values that are rounded already
+template <class T, int ALIGN>
+__device__ __forceinline__ void store_rounded(const NormArgs &a, long long row, int c, const uint32_t (&w)[4]) {
+    T *p = static_cast<T *>(a.residual_out) + row * a.cols + c;
+    if constexpr (ALIGN == 16) {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if constexpr (ALIGN == 8) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2 *>(p + 4) = make_uint2(w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (c + j < a.cols) reinterpret_cast<uint16_t *>(p)[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
     }
 }
 
@@ -170,6 +200,74 @@ __device__ __forceinline__ float group_max(float m, int group) {
     return m;
 }
 
+// Rows whose squares, or whose products with the weight, leave fp32 while the norm does not.  With the norm's factor at 2^15
+// and below, a product that is rounded as a subnormal moves y by 2^-135 at most, against scales of 2^-126 at least; above
+// that, or with a sum of squares beyond fp32, the squares are summed at `unit`^4 of their size, and y is
+// ((h * unit) * factor) * unit * weight, which leaves fp32 nowhere on the way.  Sums of two fp16 numbers are zero or between
+// 2^-24 and 2^17: no such row.
+template <class T>
+__device__ __forceinline__ bool norm_is_far(float rstd) {
+    return !std::is_same<T, __half>::value && __float_as_uint(rstd) - 1u >= __float_as_uint(0x1p15f);  // 0, above 2^15 or a NaN
+}
+// The whole row, by all threads of the block, read from memory: from an fp32 residual_out where that is `stored` (it holds
+// the sum), else from x and the residual, which residual_out has not replaced yet.
+template <class T, int ALIGN>
+__device__ __forceinline__ void norm_far_row(const NormArgs &a, long long row, bool stored, float2 (*red)[32]) {
+    const int step = blockDim.x * 8, mine = threadIdx.x * 8;
+    const auto load = [&](int c, float (&h)[8]) {
+        if (std::is_same<T, float>::value && stored) load_stored<ALIGN>(a, row, c, h);
+        else load_sum<T, ALIGN>(a, row, c, h);
+    };
+    float unit = 1.0f, rstd = 0.0f, top = 0.0f, none = 0.0f, inv = 0.0f;
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {
+        float squares = 0.0f;
+#pragma unroll 1
+        for (int c = mine; c < a.cols; c += step) {
+            float h[8];
+            load(c, h);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = h[j] * unit * unit, squares = fmaf(h[j], h[j], squares);
+        }
+        __syncthreads();
+        block_reduce(squares, none, red[turn]);
+        rstd = rsqrtf(squares * a.inv_cols + a.eps * unit * unit * unit * unit);
+        if (turn == 0) unit = !(squares <= 3.402823466e38f) ? 0x1p-48f : a.eps < 0x1p-100f && squares < 0x1p-80f ? 0x1p48f : 1.0f;
+        if (unit == 1.0f) break;
+    }
+    if (a.group == 0) {
+#pragma unroll 1
+        for (int c = mine; c < a.cols; c += step) {
+            float h[8], w[8];
+            load(c, h);
+            load_weight<ALIGN>(a, c, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = h[j] * unit * rstd * unit * w[j];
+            top = max_nan(top, largest(h));
+        }
+        __syncthreads();
+        block_reduce(none, top, red[0]);
+        const float scale = group_scale(top, a.format, inv);
+        if (threadIdx.x == 0) a.scales[row] = scale;
+    }
+#pragma unroll 1
+    for (int c = mine; c - mine < a.cols; c += step) {  // whole warps take part in the groups' shuffles
+        float h[8] = {}, w[8] = {};
+        if (c < a.cols) {
+            load(c, h);
+            load_weight<ALIGN>(a, c, w);
+            store_sum<T, ALIGN>(a, row, c, h);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = h[j] * unit * rstd * unit * w[j];
+        if (a.group != 0) {
+            const float scale = group_scale(group_max(largest(h), a.group), a.format, inv);
+            if (c < a.cols && (c & (a.group - 1)) == 0) a.scales[row * a.groups + (c >> a.group_shift)] = scale;
+        }
+        if (c < a.cols) store_q<ALIGN>(a, row, c, h, inv, inv);
+    }
+}
+
 __device__ __forceinline__ void norm_copy16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
@@ -177,16 +275,33 @@ __device__ __forceinline__ void norm_copy8(void *dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
+// Rows far from 1 are remembered (a block has NORM_ROWS at most) and done again behind the others, where their code costs
+// these no registers.  LATE: residual_out is x or the residual and of 16 bits, so that it waits until the row is known not to
+// be such a one.
+//
 // NV pieces of eight columns a thread stay in registers: blockDim.x * 8 * NV >= cols.  STAGES > 0: the block's next rows are
 // under way to shared memory while it works on this one (a thread copies what it will read itself, so no barrier orders
 // them): a row's chain of loads, two reductions and stores would leave the memory idle otherwise.
-template <class T, int ALIGN, int NV, int STAGES>
+constexpr int NORM_ROWS = 32;
+template <class T, int ALIGN, int NV, int STAGES, bool LATE>
 __global__ void __launch_bounds__(NV <= 2 && STAGES == 0 ? 1024 : 512) rmsnorm_kernel(NormArgs a) {
     constexpr int UNITS = sizeof(T) / 2;  // 16-byte pieces of eight columns
     extern __shared__ __align__(16) uint4 norm_stage[];  // [stage][x, residual][piece][unit][thread]
     __shared__ float2 red[2][32];  // in turn for odd and even rows
-    float w[8] = {};
-    if (NV == 1 && threadIdx.x * 8 < a.cols) load_weight<ALIGN>(a, threadIdx.x * 8, w);
+    // Weights stay in registers where there is room.  With many rows they are held at 2^24 of their size: inv is 2^126 at
+    // most and the factor of a row near 1 is 2^15, so that inv times 2^-24 of the factor is finite for any group.
+    constexpr bool KEEP = NV == 1 || STAGES > 0;
+    constexpr float LIFT = STAGES > 0 ? 0x1p24f : 1.0f;
+    float w[KEEP ? NV : 1][8] = {};
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * blockDim.x + threadIdx.x) * 8;
+            if (c < a.cols) load_weight<ALIGN>(a, c, w[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[i][j] *= LIFT;
+        }
+    }
     auto slot = [&](int stage, int array, int i, int u) { return norm_stage + (((stage * 2 + array) * NV + i) * UNITS + u) * blockDim.x + threadIdx.x; };
     auto prefetch = [&](long long row, int stage) {
         if (row < a.rows) {
@@ -210,9 +325,24 @@ __global__ void __launch_bounds__(NV <= 2 && STAGES == 0 ? 1024 : 512) rmsnorm_k
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    [[maybe_unused]] auto staged_sum = [&](int stage, int i, float (&h)[8]) {
+        uint4 raw[UNITS];
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) raw[u] = *slot(stage, 0, i, u);
+        load8<16>(reinterpret_cast<const T *>(raw), h);
+        if (a.residual) {
+            float f[8];
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) raw[u] = *slot(stage, 1, i, u);
+            load8<16>(reinterpret_cast<const T *>(raw), f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] += f[j];
+        }
+    };
     if constexpr (STAGES > 0)
         for (int k = 0; k < STAGES - 1; ++k) prefetch(blockIdx.x + (long long)k * gridDim.x, k);
     int stage = 0, turn = 0;
+    unsigned far_rows = 0, this_row = 1;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float h[NV][8], sum = 0.0f;
         if constexpr (STAGES > 0) {
@@ -228,66 +358,74 @@ __global__ void __launch_bounds__(NV <= 2 && STAGES == 0 ? 1024 : 512) rmsnorm_k
                 continue;
             }
             if constexpr (STAGES > 0) {
-                uint4 raw[UNITS];
-#pragma unroll
-                for (int u = 0; u < UNITS; ++u) raw[u] = *slot(stage, 0, i, u);
-                load8<16>(reinterpret_cast<const T *>(raw), h[i]);
-                if (a.residual) {
-                    float f[8];
-#pragma unroll
-                    for (int u = 0; u < UNITS; ++u) raw[u] = *slot(stage, 1, i, u);
-                    load8<16>(reinterpret_cast<const T *>(raw), f);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) h[i][j] += f[j];
-                }
+                staged_sum(stage, i, h[i]);
             } else {
                 load_sum<T, ALIGN>(a, row, c, h[i]);
             }
         }
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
         float top = 0.0f, part[NV];
+        [[maybe_unused]] uint32_t rounded[LATE && STAGES == 0 ? NV : 1][4];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
             if (c < a.cols) {
-                store_sum<T, ALIGN>(a, row, c, h[i]);
-                if (NV > 1) load_weight<ALIGN>(a, c, w);
+                if (!LATE) store_sum<T, ALIGN>(a, row, c, h[i]);
+                if (!KEEP) load_weight<ALIGN>(a, c, w[0]);
+            }
+            if constexpr (LATE && STAGES == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) rounded[i][j] = pack2(h[i][2 * j], h[i][2 * j + 1], T());
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] *= w[j];
+            for (int j = 0; j < 8; ++j) h[i][j] *= w[KEEP ? i : 0][j];
             part[i] = largest(h[i]);
             top = max_nan(top, part[i]);
         }
         turn ^= 1;
         block_reduce(sum, top, red[turn]);
         const float rstd = rsqrtf(sum * a.inv_cols + a.eps);
+        const bool far = norm_is_far<T>(rstd);
+        if (far) far_rows |= this_row;
+        this_row <<= 1;
+        const float of_product = rstd * (1.0f / LIFT);
         float inv;
         if (a.group == 0) {
-            const float scale = group_scale(top * rstd, a.format, inv);
+            const float scale = group_scale(top * of_product, a.format, inv);
             if (threadIdx.x == 0) a.scales[row] = scale;
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * blockDim.x + threadIdx.x) * 8;
             if (a.group != 0) {
-                const float scale = group_scale(group_max(part[i], a.group) * rstd, a.format, inv);
+                const float scale = group_scale(group_max(part[i], a.group) * of_product, a.format, inv);
                 if (c < a.cols && (c & (a.group - 1)) == 0) a.scales[row * a.groups + (c >> a.group_shift)] = scale;
             }
             if (c < a.cols) {
-                const float factor = code_factor(h[i], inv, rstd);
+                if constexpr (LATE && STAGES == 0)
+                    if (!far) store_rounded<T, ALIGN>(a, row, c, rounded[i]);
+                const float factor = STAGES > 0 ? inv * of_product : code_factor(h[i], inv, rstd);
                 store_q<ALIGN>(a, row, c, h[i], inv, factor);
+                if constexpr (LATE && STAGES > 0) {  // from shared memory once more: it does not fit the registers beside the weights
+                    if (!far) {
+                        staged_sum(stage, i, h[i]);
+                        store_sum<T, ALIGN>(a, row, c, h[i]);
+                    }
+                }
             }
         }
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
+    if constexpr (!std::is_same<T, __half>::value)
+        for (; far_rows; far_rows &= far_rows - 1) norm_far_row<T, ALIGN>(a, blockIdx.x + (long long)(__ffs(far_rows) - 1) * gridDim.x, a.residual_out, red);
 }
 
 // Rows that outgrow the registers: the row is read once for its sum of squares and its largest value, and once for its
 // values; residual_out is written in that second pass, so that it may be the residual (or x) itself.
 template <class T, int ALIGN>
 __global__ void __launch_bounds__(1024) rmsnorm_long_kernel(NormArgs a) {
-    __shared__ float2 red[2][32];
+    __shared__ float2 red[2][32], far_red[2][32];
     int turn = 0;
     const int step = blockDim.x * 8, spans = (a.cols + step - 1) / step;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -303,6 +441,10 @@ __global__ void __launch_bounds__(1024) rmsnorm_long_kernel(NormArgs a) {
         turn ^= 1;
         block_reduce(sum, top, red[turn]);
         const float rstd = rsqrtf(sum * a.inv_cols + a.eps);
+        if (norm_is_far<T>(rstd)) {  // nothing of the row has been stored yet
+            norm_far_row<T, ALIGN>(a, row, false, far_red);
+            continue;
+        }
         if (a.group == 0) {
             const float scale = group_scale(top * rstd, a.format, inv);
             if (threadIdx.x == 0) a.scales[row] = scale;
@@ -334,10 +476,15 @@ static int launch_norm(const NormArgs &a, int threads, const DeviceInfo *di, cud
     const size_t smem = (size_t)STAGES * 2 * NV * sizeof(T) * 8 * threads;
     int st;
     if constexpr (NV > 0) {
-        st = ensure_kernel<rmsnorm_kernel<T, ALIGN, NV, STAGES>, STAGES ? KERNEL_OPTIN_SMEM | KERNEL_MAX_CARVEOUT : 0>(di);
+        constexpr int FLAGS = STAGES ? KERNEL_OPTIN_SMEM | KERNEL_MAX_CARVEOUT : 0;
+        constexpr bool CAN_BE_LATE = std::is_same<T, __nv_bfloat16>::value;
+        const bool late = CAN_BE_LATE && a.residual_out && (a.residual_out == a.residual || a.residual_out == a.x);
+        st = late ? ensure_kernel<rmsnorm_kernel<T, ALIGN, NV, STAGES, CAN_BE_LATE>, FLAGS>(di) : ensure_kernel<rmsnorm_kernel<T, ALIGN, NV, STAGES, false>, FLAGS>(di);
         if (st) return st;
-        const int grid = (int)min((long long)a.rows, STAGES ? max(1LL, (long long)di->sm_count * (long long)(200 * 1024 / (smem + 1024))) : (long long)di->sm_count * (2048 / threads));
-        rmsnorm_kernel<T, ALIGN, NV, STAGES><<<grid, threads, smem, s>>>(a);
+        const long long resident = min((long long)a.rows, STAGES ? max(1LL, (long long)di->sm_count * (long long)(200 * 1024 / (smem + 1024))) : (long long)di->sm_count * (2048 / threads));
+        const int grid = (int)max(resident, (a.rows + NORM_ROWS - 1LL) / NORM_ROWS);
+        if (late) rmsnorm_kernel<T, ALIGN, NV, STAGES, CAN_BE_LATE><<<grid, threads, smem, s>>>(a);
+        else rmsnorm_kernel<T, ALIGN, NV, STAGES, false><<<grid, threads, smem, s>>>(a);
     } else {
         st = ensure_kernel<rmsnorm_long_kernel<T, ALIGN>, 0>(di);
         if (st) return st;
