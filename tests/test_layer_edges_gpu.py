@@ -136,3 +136,44 @@ def test_norm_of_far_rows_among_more_rows_than_a_block_remembers(lib, kind, plac
     far[[0, rows - 1]] = True
     x[far] *= 1e25
     check_far_norm(lib, x.astype(np.float64), w, kind, "int8", 32, 1e-5, residual=r.astype(np.float64), place=place)
+
+
+# ---- attention: scores whose fp32 step is more than one ------------------------------------------------------------------
+def far_scores(rng, kind, new, cached, heads, dim, q, k, requests=1):
+    p = Paged(rng, [cached] * requests, [new] * requests, heads, 1 if requests == 1 else heads, dim, 16, kind)
+    p.q_bits[:] = to_bits(np.full(p.q_bits.shape, q, np.float32), kind)
+    p.k_bits[:] = to_bits(np.full(p.k_bits.shape, k, np.float32), kind)
+    return p
+
+
+@pytest.mark.parametrize("kind,q,k", [(F16, 1000.0, 60000.0), (F16, 30000.0, 65504.0), (F16, -30000.0, 65504.0), (BF16, 2.0 ** 30, 2.0 ** 31), (BF16, 3 * 2.0 ** 29, 5 * 2.0 ** 28), (BF16, -3 * 2.0 ** 29, 5 * 2.0 ** 28)])
+@pytest.mark.parametrize("new,header", [(1, 16), (40, 16), (40, 24)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_of_huge_equal_scores_is_the_mean(lib, kind, q, k, new, header, dim):
+    """Every product is the same number, so every fp32 sum of them is too, whatever its rounding: equal weights."""
+    p = far_scores(np.random.default_rng(dim), kind, new, 300, 4, dim, q, k)
+    want, spread = p.expected()
+    u, n = HALF_STEP[kind], int(p.kv[0])
+    got = from_bits(run_attention(lib, p, header=header), kind)
+    assert np.all(np.abs(got - want) <= u * np.abs(want) + (u + (n + 8) * 2.0 ** -23) * spread + HALF_TINY[kind])
+
+
+@pytest.mark.parametrize("new,header", [(1, 16), (20, 16), (20, 24)])
+def test_attention_of_huge_scores_a_step_apart(lib, new, header):
+    """Scores of 2**27 + 16 in one key tile and 2**27 + 32 in the next one, in powers of two: a step of fp32 apart, and
+    2**-16 the weight."""
+    scale = next(float(s) for s in (np.float32(np.log(2)), np.nextafter(np.float32(np.log(2)), np.float32(1)), np.nextafter(np.float32(np.log(2)), np.float32(0)))
+                 if np.float32(s) * np.float32(1.4426950408889634) == 1.0)
+    p = far_scores(np.random.default_rng(4), F16, new, 128, 8, 64, 0.0, 0.0, requests=60)  # items that no block shares, most of them
+    p.scale = scale
+    q, k = np.zeros(64, np.float32), np.zeros(64, np.float32)
+    q[:2], k[:2] = (2.0 ** 13, 4.0), (2.0 ** 14, 4.0)
+    p.q_bits[:], p.k_bits[:] = to_bits(q, F16), to_bits(k, F16)
+    k[1] = 8.0
+    for r in range(60):
+        p.k_bits[p.table[r, 4:8]] = to_bits(k, F16)
+    got = from_bits(run_attention(lib, p, header=header), F16)
+    want, spread = p.expected()
+    u = HALF_STEP[F16]
+    # the 64-bit form's scale is ln 2 to half a step of fp32: scores of 2**27 move by 8, but alike; their difference of 16 by 2**-20
+    assert np.all(np.abs(got - want) <= u * np.abs(want) + (u + 200 * 2.0 ** -23 + 2.0 ** -19) * spread + HALF_TINY[F16])

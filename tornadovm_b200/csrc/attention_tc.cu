@@ -83,6 +83,11 @@ __device__ __forceinline__ uint32_t tc_finite_only(uint32_t w, __nv_bfloat16) {
     return ((w & 0x7F80u) == 0x7F80u ? 0u : w & 0xFFFFu) | ((w & 0x7F800000u) == 0x7F800000u ? 0u : w & 0xFFFF0000u);
 }
 
+// References from which on the step of fp32 matters.  A power of two is that of s * scale - m in one fused step, whose product
+// is not rounded; m = max s * scale is, by up to half a step, and from 2^28 on that alone takes fp16 powers beyond their
+// range.  Rows of such references round the products first.
+__device__ __forceinline__ bool tc_far(float m) { return fabsf(m) >= 0x1p20f && m != -INFINITY; }
+
 struct TcShared {
     uint64_t kv_full[10], kv_empty[10];
     uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drained[2];  // [row tile][score buffer]
@@ -368,6 +373,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const int lead = min(2, im.ntiles);
             pv_use += lead - 1;  // an item of two tiles or more commits the last product but one
             float m = -INFINITY, l = 0.0f;
+            bool far = false;
 #pragma unroll 1
             for (int n = 0; n < im.ntiles; ++n, ++nkv, ++nslot, ++g) {
                 const uint32_t b = g & 1;
@@ -426,25 +432,33 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     fence_async_shared();
                 }
                 if (warp_has) {
-                    if (n == 0) m = top;
-                    if (__builtin_expect(__any_sync(0xffffffffu, top > m + 8.0f), 0)) {
-                        // The product before this one may still be adding to O.  The next scores' product follows it; behind
-                        // the last scores it has a barrier of its own.
-                        ok = __all_sync(0xffffffffu, n + 1 < im.ntiles ? mbar_wait_abortable(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1, abortp)
-                                                                       : mbar_wait_abortable(&sh.pv_done[t], (pv_use - 1) & 1, abortp));
-                        if (!ok) break;
-                        tc_fence_after();
-                        const float next = fmaxf(m, top), f = next == m ? 1.0f : tc_ex2(m - next);
+                    uint64_t by = scale2;
+                    if (n == 0) m = top, far = tc_far(m);
+                    if (__builtin_expect(__any_sync(0xffffffffu, top - m > 8.0f || far), 0)) {
+                        if (__any_sync(0xffffffffu, top - m > 8.0f)) {
+                            // The product before this one may still be adding to O.  The next scores' product follows it; behind
+                            // the last scores it has a barrier of its own.
+                            ok = __all_sync(0xffffffffu, n + 1 < im.ntiles ? mbar_wait_abortable(&sh.s_full[t][b ^ 1], ((g + 1) >> 1) & 1, abortp)
+                                                                           : mbar_wait_abortable(&sh.pv_done[t], (pv_use - 1) & 1, abortp));
+                            if (!ok) break;
+                            tc_fence_after();
+                            const float next = fmaxf(m, top), f = next == m ? 1.0f : tc_ex2(m - next);
 #pragma unroll 1
-                        for (int c = 0; c < DPAD / 32; ++c) {
-                            uint32_t o[32];
-                            tc_ld_32cols(o_addr + c * 32, o);
-                            tc_wait_ld();
+                            for (int c = 0; c < DPAD / 32; ++c) {
+                                uint32_t o[32];
+                                tc_ld_32cols(o_addr + c * 32, o);
+                                tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tc_st_32cols(o_addr + c * 32, o);
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tc_st_32cols(o_addr + c * 32, o);
+                            }
+                            l *= f, m = next, far = tc_far(m);
                         }
-                        l *= f, m = next;
+                        if (__any_sync(0xffffffffu, far)) {  // rounded like `top`, so that the difference to m is exact
+#pragma unroll
+                            for (int i = 0; i < 64; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * a.scale_log2);
+                            by = tc_pair(1.0f, 1.0f);
+                        }
                     }
                     const float shift = m == -INFINITY ? 0.0f : -m;
                     const uint64_t shift2 = tc_pair(shift, shift);
@@ -453,7 +467,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         float p0, p1;
-                        tc_split(tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift2), p0, p1);
+                        tc_split(tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), by, shift2), p0, p1);
                         p0 = tc_ex2(p0), p1 = tc_ex2(p1);
                         sum[i & 1] = tc_add2(sum[i & 1], tc_pair(p0, p1));
                         p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
