@@ -177,3 +177,32 @@ def test_attention_of_huge_scores_a_step_apart(lib, new, header):
     u = HALF_STEP[F16]
     # the 64-bit form's scale is ln 2 to half a step of fp32: scores of 2**27 move by 8, but alike; their difference of 16 by 2**-20
     assert np.all(np.abs(got - want) <= u * np.abs(want) + (u + 200 * 2.0 ** -23 + 2.0 ** -19) * spread + HALF_TINY[F16])
+
+
+# ---- attention: a long flat tail far below one large score ---------------------------------------------------------------
+@pytest.mark.parametrize("requests,new,header", [(60, 1, 16), (20, 20, 16), (20, 20, 24)])
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("gap", [12.0, 16.9, 17.6])
+def test_attention_keeps_a_tail_of_small_probabilities(lib, requests, new, header, kind, gap):
+    """One key takes nearly all of the weight and has V = 0; the result is what thousands of keys at e**-gap of it have.
+    An fp16 probability is held to half a step of the type down to 2**-14 of the largest one at least, and below that to
+    2**-25 times what the probabilities are raised by before the rounding (2**7 at least)."""
+    rng = np.random.default_rng(requests)
+    cached, heads, dim = 2000, 8, 64
+    p = Paged(rng, [cached] * requests, [new] * requests, heads, heads, dim, 16, kind)
+    p.scale = 0.125
+    p.q_bits[:] = to_bits(np.full(p.q_bits.shape, 1.0, np.float32), kind)
+    low = to_bits(np.full(p.k_bits.shape, 1.0, np.float32), kind)
+    p.k_bits[:] = low
+    p.v_bits[:] = to_bits(1 + 0.25 * rng.random(p.v_bits.shape), kind)
+    first = np.full(dim, 1.0, np.float32)
+    first[:8] += gap  # 8 * gap / 8: exact in both types where gap + 1 is
+    for r in range(requests):
+        p.k_bits[p.table[r, 0], :, 0], p.v_bits[p.table[r, 0], :, 0] = to_bits(first, kind), 0
+    got = from_bits(run_attention(lib, p, header=header), kind)
+    want, spread = p.expected()
+    u, n = HALF_STEP[kind], cached + new
+    ds = (dim + 2) * 2.0 ** -23 * 8.0 * np.sqrt((from_bits(to_bits(first, kind), kind) ** 2).sum()) * p.scale
+    tail = n * HALF_TINY[kind] * 2.0 ** -7 * 1.25
+    tol = u * np.abs(want) + (1 + u) * (u + 2 * ds + (n + 8) * 2.0 ** -23) * spread + tail + HALF_TINY[kind]
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) - tol)

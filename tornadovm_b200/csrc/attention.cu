@@ -57,6 +57,13 @@ __device__ __forceinline__ void at_mma(float (&d)[4], const uint32_t (&a)[4], ui
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// What is taken off a row's scores: their maximum.  bf16 has fp32's exponents.  An fp16 power is a subnormal below 2^-14, off
+// by up to 2^-25, and vanishes from the product with V, though not from the sum, below that: the powers are raised by 2^15 (of
+// fp16's 2^16), which the sum and O share, so that a long tail of small probabilities is held to 2^-40 of the largest one.
+// Not where a step of fp32 could lift them further.
+__device__ __forceinline__ float at_shift(float m, __nv_bfloat16) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ float at_shift(float m, __half) { return m == -INFINITY ? 0.0f : fabsf(m) < 0x1p20f ? m - 15.0f : m; }
+
 template <int DPAD, bool SPLIT_KEYS>
 struct AtShape {
     static constexpr int ROWS = SPLIT_KEYS ? 16 : 64;
@@ -262,10 +269,10 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
                     top[h] = fmaxf(top[h], m[h]);
-                    shift[h] = top[h] == -INFINITY ? 0.0f : top[h];
+                    shift[h] = at_shift(top[h], T());
                 }
                 if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
-                    const float f0 = ex2(m[0] - shift[0]), f1 = ex2(m[1] - shift[1]);
+                    const float f0 = m[0] == -INFINITY ? 0.0f : ex2(at_shift(m[0], T()) - shift[0]), f1 = m[1] == -INFINITY ? 0.0f : ex2(at_shift(m[1], T()) - shift[1]);
                     l[0] *= f0, l[1] *= f1;
 #pragma unroll
                     for (int n = 0; n < DPAD / 8; ++n) o[n][0] *= f0, o[n][1] *= f0, o[n][2] *= f1, o[n][3] *= f1;
@@ -297,7 +304,7 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
                             const float p0 = ex2(s[2 * n + h][0] - shift[0]), p1 = ex2(s[2 * n + h][1] - shift[0]);
                             const float p2 = ex2(s[2 * n + h][2] - shift[1]), p3 = ex2(s[2 * n + h][3] - shift[1]);
                             l[0] += p0 + p1, l[1] += p2 + p3;
-                            p[2 * h] = pack2(p0, p1, T()), p[2 * h + 1] = pack2(p2, p3, T());  // half a step of `type`, relative to p
+                            p[2 * h] = pack2(p0, p1, T()), p[2 * h + 1] = pack2(p2, p3, T());  // half a step of `type`, relative to p (fp16: 2^-25 below 2^-14)
                         }
 #pragma unroll
                         for (int d = 0; d < DPAD / 16; ++d) {
@@ -373,7 +380,7 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int row = lane / 4 + 8 * h;
-                if ((lane & 3) == 0) ml[(warp * 16 + row) * 2] = m[h], ml[(warp * 16 + row) * 2 + 1] = l[h];
+                if ((lane & 3) == 0) ml[(warp * 16 + row) * 2] = at_shift(m[h], T()), ml[(warp * 16 + row) * 2 + 1] = l[h];
 #pragma unroll
                 for (int n = 0; n < DPAD / 8; ++n)
                     *reinterpret_cast<float2 *>(acc + (warp * 16 + row) * DPAD + 8 * n + 2 * (lane & 3)) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
@@ -406,7 +413,7 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
                     const float inv = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
 #pragma unroll
                     for (int n = 0; n < DPAD / 8; ++n) put(row, 8 * n + 2 * (lane & 3), o[n][2 * h], o[n][2 * h + 1], inv);
-                    if (!whole && (lane & 3) == 0) part[row * attn_part_pitch(DPAD) + DPAD] = m[h], part[row * attn_part_pitch(DPAD) + DPAD + 1] = l[h];
+                    if (!whole && (lane & 3) == 0) part[row * attn_part_pitch(DPAD) + DPAD] = at_shift(m[h], T()), part[row * attn_part_pitch(DPAD) + DPAD + 1] = l[h];
                 }
             }
         }

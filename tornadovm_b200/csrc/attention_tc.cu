@@ -11,8 +11,8 @@
 //   * warp 11 fetches the query rows;
 //   * warps 0-3 and 4-7 hold the softmax of one 128-row tile each, a row per thread: S from tensor memory, the running
 //     maximum and sum in registers, P back as 16-bit values.  O stays in tensor memory; it is rescaled only when a row's
-//     maximum has grown by more than 2^8 since its reference was set (P then reaches 256 at most, well inside fp16, and
-//     the quotient O / l does not depend on the reference), which after the first tiles of a row hardly ever happens.
+//     maximum has grown by more than 2^8 since its reference was set (P then reaches 2^8 at most, 2^15 as
+//     fp16 holds it, and the quotient O / l does not depend on the reference), which after the first tiles of a row hardly ever happens.
 // Bound: per row tile and key tile two products of 128 x 64 x head_dim, and 128 x 64 powers of two.  The key tiles of all
 // items are divided evenly over the blocks and split rows are joined afterwards (attention.cuh).  Code that runs once an
 // item stays in rolled loops: unrolled, its instructions arrived from L2 at 15 cycles each (fetching the query rows took
@@ -87,6 +87,13 @@ __device__ __forceinline__ uint32_t tc_finite_only(uint32_t w, __nv_bfloat16) {
 // is not rounded; m = max s * scale is, by up to half a step, and from 2^28 on that alone takes fp16 powers beyond their
 // range.  Rows of such references round the products first.
 __device__ __forceinline__ bool tc_far(float m) { return fabsf(m) >= 0x1p20f && m != -INFINITY; }
+
+// What is taken off a row's scores.  bf16 has fp32's exponents.  An fp16 power is a subnormal below 2^-14, off by up to 2^-25,
+// and vanishes from P, though not from the sum, below that: P is raised by 2^7 (2^8 over the reference it reaches 2^15, of
+// 2^16), which the sum and O share, so that a long tail of small probabilities is held to 2^-32 of the largest one.  Not
+// where a step of fp32 could lift it further.
+__device__ __forceinline__ float tc_shift(float m, __nv_bfloat16) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ float tc_shift(float m, __half) { return m == -INFINITY ? 0.0f : tc_far(m) ? m : m - 7.0f; }
 
 struct TcShared {
     uint64_t kv_full[10], kv_empty[10];
@@ -442,7 +449,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                                                                            : mbar_wait_abortable(&sh.pv_done[t], (pv_use - 1) & 1, abortp));
                             if (!ok) break;
                             tc_fence_after();
-                            const float next = fmaxf(m, top), f = next == m ? 1.0f : tc_ex2(m - next);
+                            const float next = fmaxf(m, top), f = next == m ? 1.0f : m == -INFINITY ? 0.0f : tc_ex2(tc_shift(m, T()) - tc_shift(next, T()));
 #pragma unroll 1
                             for (int c = 0; c < DPAD / 32; ++c) {
                                 uint32_t o[32];
@@ -460,7 +467,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                             by = tc_pair(1.0f, 1.0f);
                         }
                     }
-                    const float shift = m == -INFINITY ? 0.0f : -m;
+                    const float shift = -tc_shift(m, T());
                     const uint64_t shift2 = tc_pair(shift, shift);
                     uint64_t sum[2] = {0, 0};
                     uint32_t p[32];
@@ -470,7 +477,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         tc_split(tc_fma2(tc_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), by, shift2), p0, p1);
                         p0 = tc_ex2(p0), p1 = tc_ex2(p1);
                         sum[i & 1] = tc_add2(sum[i & 1], tc_pair(p0, p1));
-                        p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p
+                        p[i] = pack2(p0, p1, T());  // half a step of `type`, relative to p (fp16: 2^-25 below 2^-14)
                     }
                     tc_st_32cols(s_addr + b * 64, p);
                     float s0, s1;
@@ -536,7 +543,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         }
                     }
                 }
-                if (!whole) part[DPAD * ROWS] = m, part[(DPAD + 1) * ROWS] = l;
+                if (!whole) part[DPAD * ROWS] = tc_shift(m, T()), part[(DPAD + 1) * ROWS] = l;
             }
             if (threadIdx.x == 0) {
                 if (!whole && done.from == 0)
