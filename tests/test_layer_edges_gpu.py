@@ -206,3 +206,16 @@ def test_attention_keeps_a_tail_of_small_probabilities(lib, requests, new, heade
     tail = n * HALF_TINY[kind] * 2.0 ** -7 * 1.25
     tol = u * np.abs(want) + (1 + u) * (u + 2 * ds + (n + 8) * 2.0 ** -23) * spread + tail + HALF_TINY[kind]
     assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) - tol)
+
+
+# ---- attention: nothing but scores of minus infinity ---------------------------------------------------------------------
+@pytest.mark.parametrize("value", [np.inf, np.nan])
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("cached,new,header", [(40, 1, 16), (40, 3, 16), (100, 40, 16), (100, 40, 24), (5000, 1, 16), (5000, 40, 16)])
+def test_attention_rows_of_minus_infinity_are_zeros_whatever_their_values(lib, value, kind, cached, new, header):
+    rng = np.random.default_rng(cached + new)
+    p = Paged(rng, [cached], [new], 4, 2, 64, 16, kind)
+    p.q_bits[:] = to_bits(np.abs(from_bits(p.q_bits, kind)) + 0.1, kind)
+    p.k_bits[:] = to_bits(np.float32(-np.inf), kind)
+    p.v_bits[:, :, ::3] = to_bits(np.float32(value), kind)
+    assert np.all(run_attention(lib, p, header=header)[:new] == 0)

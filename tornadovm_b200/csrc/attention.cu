@@ -411,6 +411,10 @@ __global__ void __launch_bounds__(AT_THREADS, AtShape<DPAD, SPLIT_KEYS>::BLOCKS_
                 const int row = my_row + 8 * h;
                 if (row < rows) {
                     const float inv = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
+                    if (__builtin_expect(l[h] == 0.0f, 0)) {  // saw nothing, or only scores of -infinity, times values that need not be finite
+#pragma unroll
+                        for (int n = 0; n < DPAD / 8; ++n) o[n][2 * h] = o[n][2 * h + 1] = 0.0f;
+                    }
 #pragma unroll
                     for (int n = 0; n < DPAD / 8; ++n) put(row, 8 * n + 2 * (lane & 3), o[n][2 * h], o[n][2 * h + 1], inv);
                     if (!whole && (lane & 3) == 0) part[row * attn_part_pitch(DPAD) + DPAD] = at_shift(m[h], T()), part[row * attn_part_pitch(DPAD) + DPAD + 1] = l[h];

@@ -528,6 +528,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                             }
                         }
                     }
+                    if (__builtin_expect(l == 0.0f, 0)) {  // saw nothing, or only scores of -infinity, times values that need not be finite
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = 0;
+                    }
                     if (!whole) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) part[(c * 32 + i) * ROWS] = __uint_as_float(o[i]);
