@@ -443,7 +443,8 @@ int tb200_rmsnorm_quant(int rows, int cols, int type, const void *x, long long x
  * A request gets only the new tokens that its table row (max_pages * page_size positions) and the max_tokens rows
  * hold: cu_new and kv_lens say how many, counts[0] < counts[1] says that some did not fit.  When free_pages runs out
  * (counts[2] < counts[3]) the entries of the missing pages and the slots of their tokens are -1.  Entries that the step
- * does not add are left as they were.  requests <= 16384, max_tokens <= 2^30, max_pages * page_size <= 2^30. */
+ * does not add are left as they were.  What is written must not overlap any other array of the call (kv_lens not
+ * cached_lens either: two arrays in turn).  requests <= 16384, max_tokens <= 2^30, max_pages * page_size <= 2^30. */
 int tb200_paged_plan(int requests, int page_size, int max_pages, int max_tokens, int num_free, const int32_t *cached_lens,
                      const int32_t *new_lens, const int32_t *free_pages, int32_t *block_table, int32_t *cu_new, int32_t *kv_lens,
                      int32_t *positions, int64_t *slots, int32_t *counts, tb200_stream_t stream);

@@ -264,6 +264,12 @@ public final class B200 {
         check(maxTokens >= 0 && maxTokens <= 1 << 30, "B200 pagedPlan requires 0 <= maxTokens <= 2^30; got " + maxTokens);
         check(cachedLens.getSize() >= requests && newLens.getSize() >= requests && blockTable.getSize() >= (long) requests * maxPages && cuNew.getSize() >= requests + 1
                 && kvLens.getSize() >= requests && positions.getSize() >= maxTokens && slots.getSize() >= maxTokens && counts.getSize() >= 4, "B200 pagedPlan: array too small");
+        Object[] arrays = { blockTable, cuNew, kvLens, positions, slots, counts, cachedLens, newLens, freePages };
+        for (int i = 0; i < 6; i++) {
+            for (int j = i + 1; j < arrays.length; j++) {
+                check(arrays[i] != arrays[j], "B200 pagedPlan: an output and another array of the task are one array");
+            }
+        }
         return descriptor("pagedPlan", new Object[] { requests, pageSize, maxPages, maxTokens, freePages.getSize(), cachedLens, newLens, freePages, blockTable, cuNew, kvLens, positions, slots,
                 counts }, new int[] { 8 }, new int[] { 9, 10, 11, 12, 13 });
     }

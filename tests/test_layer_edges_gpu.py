@@ -1,8 +1,12 @@
 """Ends of the decoder-layer operators' ranges on the GPU: hints that are too small, windows without an end, values near
 the ends of fp32, scores whose step is more than one, probabilities far below the largest one."""
+import ctypes as C
+
 import numpy as np
 import pytest
+import torch
 
+from harness import stream_ptr, sync_and_check
 from layer_util import BF16, F16, F32, HALF_STEP, HALF_TINY, Paged, fp8_values, from_bits, to_bits
 from oracle import layer as ol
 from test_layer_gpu import check_attention, run_attention, run_norm
@@ -219,3 +223,29 @@ def test_attention_rows_of_minus_infinity_are_zeros_whatever_their_values(lib, v
     p.k_bits[:] = to_bits(np.float32(-np.inf), kind)
     p.v_bits[:, :, ::3] = to_bits(np.float32(value), kind)
     assert np.all(run_attention(lib, p, header=header)[:new] == 0)
+
+
+# ---- plan: arrays that lie next to one another ----------------------------------------------------------------------------
+def test_plan_of_neighbouring_arrays_and_shared_lengths(lib):
+    """Only an output over another array is refused: kv_lens may begin where cached_lens ends, and both lengths may be one
+    array."""
+    n, page, width, rows = 3, 4, 5, 16
+    lens, free = np.array([3, 0, 6], np.int32), np.arange(10, 16, dtype=np.int32)
+    table = np.arange(n * width, dtype=np.int32).reshape(n, width)
+    want = ol.paged_plan(lens, lens, page, width, rows, free, table)
+    b = torch.zeros(512, dtype=torch.int32, device="cuda")
+    places, at = {}, 0
+    for name, size in (("slots", 2 * rows), ("cached", n), ("kv", n), ("cu", n + 1), ("counts", 4), ("positions", rows), ("free", len(free)), ("table", n * width)):
+        places[name], at = (at, size), at + size
+    host = b.cpu().numpy()
+    host[places["cached"][0]:][:n], host[places["free"][0]:][:len(free)], host[places["table"][0]:][:n * width] = lens, free, table.ravel()
+    b.copy_(torch.from_numpy(host))
+    P = lambda k: C.c_void_p(b.data_ptr() + 4 * places[k][0])  # noqa: E731
+    assert lib.tb200_paged_plan(n, page, width, rows, len(free), P("cached"), P("cached"), P("free"), P("table"), P("cu"), P("kv"), P("positions"), P("slots"), P("counts"),
+                                stream_ptr()) == 0
+    sync_and_check(lib)
+    got = b.cpu().numpy()
+    take = lambda k: got[places[k][0]:][:places[k][1]]  # noqa: E731
+    assert np.array_equal(take("table").reshape(n, width), want[0]) and np.array_equal(take("slots").view(np.int64), want[4])
+    for k, w in (("cu", want[1]), ("kv", want[2]), ("positions", want[3]), ("counts", want[5])):
+        assert np.array_equal(take(k), w), k

@@ -2,7 +2,7 @@
 anything is launched (no GPU needed)."""
 import pytest
 
-from test_layer_cpu import INVALID, P, attention, norm
+from test_layer_cpu import INVALID, P, attention, norm, plan
 
 
 @pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) - 8192, (1 << 31) - 1])
@@ -28,3 +28,32 @@ def test_factories_refuse_what_the_library_refuses():
     k = h(2 * 16 * 64)
     with pytest.raises(RuntimeError, match="requests <= 2"):
         B200.pagedAttention(1, (1 << 30) + 1, 0, 4, 2, 64, h(256), IntArray(2), IntArray(1), IntArray(1), 16, k, k, 0.1, 0, h(256))
+
+
+def plan_places(**kw):
+    """Arrays of a plan for two requests behind one another, 256 bytes each."""
+    names = ("cached", "new", "free", "table", "cu", "kv", "positions", "slots", "counts")
+    return {n: P + 256 * i for i, n in enumerate(names)} | kw
+
+
+@pytest.mark.parametrize("out,on,by", [("kv", "cached", 0), ("kv", "new", 0), ("kv", "cached", 4), ("cu", "new", -8), ("cu", "cached", 4), ("positions", "new", 4), ("slots", "cached", 0),
+                                       ("counts", "new", -12), ("table", "free", 8), ("table", "cached", 4), ("kv", "cu", 8), ("positions", "slots", 60), ("counts", "positions", 0),
+                                       ("kv", "counts", 12), ("slots", "table", 24)])
+def test_plan_refuses_outputs_over_other_arrays(lib, out, on, by):
+    """Every block reads the lengths for itself while the first one writes kv_lens: updating them in place is a race, and
+    so is any other output over an array that the call reads or writes."""
+    at = plan_places()
+    assert plan(lib, **(at | {out: at[on] + by})) == INVALID
+
+
+def test_plan_factory_refuses_outputs_over_other_arrays():
+    from tornadovm_b200.arrays import IntArray as I, LongArray
+    from tornadovm_b200.b200 import B200
+    a = dict(requests=2, pageSize=16, maxPages=4, maxTokens=8, cachedLens=I(2), newLens=I(2), freePages=I(3), blockTable=I(8), cuNew=I(3), kvLens=I(2), positions=I(8),
+             slots=LongArray(8), counts=I(4))
+    B200.pagedPlan(**a)
+    B200.pagedPlan(**(a | dict(newLens=a["cachedLens"])))
+    a |= dict(counts=I(4), freePages=I(4))
+    for kw in (dict(kvLens=a["cachedLens"]), dict(cuNew=a["positions"]), dict(counts=a["freePages"]), dict(blockTable=a["positions"])):
+        with pytest.raises(RuntimeError, match="one array"):
+            B200.pagedPlan(**(a | kw))

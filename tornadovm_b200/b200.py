@@ -271,6 +271,8 @@ class B200:
         _check(cachedLens.getSize() >= requests and newLens.getSize() >= requests and blockTable.getSize() >= requests * maxPages
                and cuNew.getSize() >= requests + 1 and kvLens.getSize() >= requests and positions.getSize() >= maxTokens
                and slots.getSize() >= maxTokens and counts.getSize() >= 4, "B200 pagedPlan: array too small")
+        arrays = (blockTable, cuNew, kvLens, positions, slots, counts, cachedLens, newLens, freePages)
+        _check(not any(out is other for i, out in enumerate(arrays[:6]) for other in arrays[i + 1:]), "B200 pagedPlan: an output and another array of the task are one array")
         params = [requests, pageSize, maxPages, maxTokens, freePages.getSize(), cachedLens, newLens, freePages, blockTable, cuNew, kvLens, positions, slots, counts]
         return _desc("pagedPlan", params, {8: Access.READ_WRITE} | {i: Access.WRITE_ONLY for i in range(9, 14)})
 

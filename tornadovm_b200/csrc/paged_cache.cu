@@ -355,6 +355,15 @@ extern "C" int tb200_paged_plan(int requests, int page_size, int max_pages, int 
     for (const void *p : words)
         if (!aligned_to(p, 4)) return TB200_ERR_ALIGNMENT;
     if (!aligned_to(slots, 8)) return TB200_ERR_ALIGNMENT;
+    // Blocks read the lengths and the free list while others write: an output over another array would be a race.
+    const long long R = requests;
+    const struct { const void *at; long long bytes; } arrays[] = {{block_table, R * max_pages * 4}, {cu_new, (R + 1) * 4}, {kv_lens, R * 4}, {positions, max_tokens * 4LL},
+                                                                   {slots, max_tokens * 8LL}, {counts, 16}, {cached_lens, R * 4}, {new_lens, R * 4}, {free_pages, num_free * 4LL}};
+    for (int i = 0; i < 6; ++i)  // the outputs
+        for (int j = i + 1; j < 9; ++j) {
+            const uintptr_t a = (uintptr_t)arrays[i].at, b = (uintptr_t)arrays[j].at;
+            if (arrays[i].bytes > 0 && arrays[j].bytes > 0 && a < b + arrays[j].bytes && b < a + arrays[i].bytes) return TB200_ERR_INVALID_ARG;
+        }
     int st;
     const DeviceInfo *di = device_info(&st);
     if (!di) return st;
