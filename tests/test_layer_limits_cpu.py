@@ -12,6 +12,12 @@ def test_norm_refuses_rows_that_32_bits_do_not_index(lib, cols):
         assert norm(lib, cols=cols, x_stride=1 << 31, **kw) == INVALID
 
 
+def test_norm_refuses_a_sum_over_x_at_another_pitch(lib):
+    """residual_out's rows are cols apart: over an x whose rows are not, they would land on rows that are still to be read."""
+    assert norm(lib, x=P, residual_out=P, x_stride=72) == INVALID
+    assert norm(lib, x=P, residual=None, residual_out=P, x_stride=65, type=0) == INVALID
+
+
 def test_attention_refuses_requests_that_32_bits_do_not_index(lib):
     for requests in ((1 << 30) + 1, (1 << 31) - 1):
         assert attention(lib, requests=requests) == INVALID

@@ -529,7 +529,7 @@ extern "C" int tb200_rmsnorm_quant(int rows, int cols, int type, const void *x, 
     if (format < TB200_Q_INT8 || format > TB200_Q_E5M2 || !(group == 0 || group == 32 || group == 64 || group == 128)) return TB200_ERR_INVALID_ARG;
     if (!(eps >= 0.0f) || eps > 3.402823466e38f) return TB200_ERR_INVALID_ARG;
     if (rows == 0) return TB200_OK;
-    if (!x || !weight || !q || !scales) return TB200_ERR_INVALID_ARG;
+    if (!x || !weight || !q || !scales || (residual_out == x && x_stride != cols && rows > 1)) return TB200_ERR_INVALID_ARG;
     const uintptr_t b = (uintptr_t)type_bytes(type);
     if (!aligned_to(x, b) || (residual && !aligned_to(residual, b)) || (residual_out && !aligned_to(residual_out, b)) || !aligned_to(weight, 4) ||
         !aligned_to(scales, 4))
