@@ -280,15 +280,20 @@ extern "C" int tb200_device_status_of(int op_classes, int *status_out) {
     constexpr int kReaders = sizeof(readers) / sizeof(readers[0]);
     // One word per translation unit: the reads are enqueued together into pinned memory and waited for once (a
     // host class calls this after every step; eight blocking copies cost more than the step's launch).
+    // Pinned memory ends with the context that it was allocated in, so each context has its own.
+    int st;
+    const DeviceInfo *di = device_info(&st);
+    if (!di) return st;
     static std::mutex mutex;
-    static int *pinned = nullptr;
+    static int *words[kMaxContexts] = {};
     std::lock_guard<std::mutex> lock(mutex);
-    if (!pinned) {
+    if (!words[di->slot]) {
         void *p = nullptr;
-        cudaError_t e = cudaHostAlloc(&p, kReaders * sizeof(int), cudaHostAllocPortable);
+        cudaError_t e = cudaHostAlloc(&p, kReaders * sizeof(int), cudaHostAllocDefault);
         if (e != cudaSuccess) return (int)e;
-        pinned = static_cast<int *>(p);
+        words[di->slot] = static_cast<int *>(p);
     }
+    int *pinned = words[di->slot];
     if (op_classes == 0) op_classes = TB200_PREPARE_ALL;
     bool selected[kReaders];
     for (int i = 0; i < kReaders; ++i) {
@@ -296,7 +301,7 @@ extern "C" int tb200_device_status_of(int op_classes, int *status_out) {
         selected[i] = r.op_class != TB200_PREPARE_ALL ? (r.op_class & op_classes) != 0 : op_classes == TB200_PREPARE_ALL;
         pinned[i] = 0;
         if (selected[i]) {
-            const int st = r.read_async(pinned + i);
+            st = r.read_async(pinned + i);
             if (st) return st;
         }
     }
@@ -306,7 +311,7 @@ extern "C" int tb200_device_status_of(int op_classes, int *status_out) {
     for (int i = 0; i < kReaders; ++i) {
         if (!selected[i] || pinned[i] == 0) continue;
         if (combined == 0) combined = pinned[i];
-        const int st = readers[i].clear();  // read and clear, like cudaGetLastError
+        st = readers[i].clear();  // read and clear, like cudaGetLastError
         if (st) return st;
     }
     *status_out = combined;
