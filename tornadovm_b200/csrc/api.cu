@@ -5,40 +5,21 @@
 
 #include "common.cuh"
 
-TB200_TU_STATUS(api)
-
 namespace tb200 {
 
-// status readers of the other translation units (TB200_TU_STATUS in each)
-int tu_status_gemv_f32(int *);
-int tu_status_gemv_quant(int *);
-int tu_status_gemv_mma(int *);
-int tu_status_gemv_tc(int *);
-int tu_status_sgemm(int *);
-int tu_status_hgemm(int *);
-int tu_status_peer(int *);
-int tu_status_read_async_api(int *);
-int tu_status_clear_api();
+// status readers of the translation units that have something to report (TB200_TU_STATUS in each)
 int tu_status_read_async_gemv_f32(int *);
 int tu_status_clear_gemv_f32();
 int tu_status_read_async_gemv_quant(int *);
 int tu_status_clear_gemv_quant();
-int tu_status_read_async_gemv_mma(int *);
-int tu_status_clear_gemv_mma();
 int tu_status_read_async_gemv_tc(int *);
 int tu_status_clear_gemv_tc();
-int tu_status_read_async_sgemm(int *);
-int tu_status_clear_sgemm();
 int tu_status_read_async_hgemm(int *);
 int tu_status_clear_hgemm();
 int tu_status_read_async_peer(int *);
 int tu_status_clear_peer();
-int tu_status_read_async_rmsnorm(int *);
-int tu_status_clear_rmsnorm();
 int tu_status_read_async_paged_cache(int *);
 int tu_status_clear_paged_cache();
-int tu_status_read_async_attention(int *);
-int tu_status_clear_attention();
 int tu_status_read_async_attention_tc(int *);
 int tu_status_clear_attention_tc();
 
@@ -265,21 +246,17 @@ extern "C" int tb200_device_status_of(int op_classes, int *status_out) {
         int (*clear)();
         int op_class;
     };
-    static const Reader readers[] = {{tu_status_read_async_api, tu_status_clear_api, TB200_PREPARE_ALL},
-                                     {tu_status_read_async_gemv_f32, tu_status_clear_gemv_f32, TB200_PREPARE_GEMV_F32},
+    // the units whose kernels wait for something or check positions; the others have nothing to report, and a read costs 3 us
+    static const Reader readers[] = {{tu_status_read_async_gemv_f32, tu_status_clear_gemv_f32, TB200_PREPARE_GEMV_F32},
                                      {tu_status_read_async_gemv_quant, tu_status_clear_gemv_quant, TB200_PREPARE_GEMV_QUANT},
-                                     {tu_status_read_async_gemv_mma, tu_status_clear_gemv_mma, TB200_PREPARE_GEMV_QUANT},
                                      {tu_status_read_async_gemv_tc, tu_status_clear_gemv_tc, TB200_PREPARE_GEMV_QUANT},
-                                     {tu_status_read_async_sgemm, tu_status_clear_sgemm, TB200_PREPARE_GEMM_F32},
                                      {tu_status_read_async_hgemm, tu_status_clear_hgemm, TB200_PREPARE_GEMM_F16},
                                      {tu_status_read_async_peer, tu_status_clear_peer, TB200_PREPARE_PEER},
-                                     {tu_status_read_async_rmsnorm, tu_status_clear_rmsnorm, TB200_PREPARE_LAYER},
                                      {tu_status_read_async_paged_cache, tu_status_clear_paged_cache, TB200_PREPARE_LAYER},
-                                     {tu_status_read_async_attention, tu_status_clear_attention, TB200_PREPARE_LAYER},
                                      {tu_status_read_async_attention_tc, tu_status_clear_attention_tc, TB200_PREPARE_LAYER}};
     constexpr int kReaders = sizeof(readers) / sizeof(readers[0]);
-    // One word per translation unit: the reads are enqueued together into pinned memory and waited for once (a
-    // host class calls this after every step; eight blocking copies cost more than the step's launch).
+    // One word per unit: the reads are enqueued together into pinned memory and waited for once (a
+    // host class calls this after every step; as many blocking copies cost more than the step's launch).
     // Pinned memory ends with the context that it was allocated in, so each context has its own.
     int st;
     const DeviceInfo *di = device_info(&st);
@@ -298,7 +275,7 @@ extern "C" int tb200_device_status_of(int op_classes, int *status_out) {
     bool selected[kReaders];
     for (int i = 0; i < kReaders; ++i) {
         const Reader &r = readers[i];
-        selected[i] = r.op_class != TB200_PREPARE_ALL ? (r.op_class & op_classes) != 0 : op_classes == TB200_PREPARE_ALL;
+        selected[i] = (r.op_class & op_classes) != 0;
         pinned[i] = 0;
         if (selected[i]) {
             st = r.read_async(pinned + i);

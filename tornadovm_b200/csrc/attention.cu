@@ -13,8 +13,6 @@
 #define TB200_OP_CLASS TB200_PREPARE_LAYER
 #include "attention.cuh"
 
-TB200_TU_STATUS(attention)
-
 namespace tb200 {
 
 constexpr int AT_THREADS = 128, AT_KEYS = 64;

@@ -19,8 +19,6 @@
 #define TB200_OP_CLASS TB200_PREPARE_GEMV_QUANT
 #include "gemv_common.cuh"
 
-TB200_TU_STATUS(gemv_mma)
-
 namespace tb200 {
 
 constexpr int MM_WARPS = 8 /* 16-row units per round */, MM_KSPLIT = 2 /* warps per unit */;

@@ -24,8 +24,6 @@
 #define TB200_OP_CLASS TB200_PREPARE_LAYER
 #include "layer_common.cuh"
 
-TB200_TU_STATUS(rmsnorm)
-
 namespace tb200 {
 
 struct NormArgs {

@@ -14,8 +14,6 @@
 #include "common.cuh"
 #include "gemm_generic.cuh"
 
-TB200_TU_STATUS(sgemm)
-
 namespace tb200 {
 
 constexpr int SG_BM = 128, SG_BN = 128, SG_BK = 16, SG_THREADS = 256;
