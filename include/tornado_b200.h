@@ -456,7 +456,7 @@ int tb200_paged_plan(int requests, int page_size, int max_pages, int max_tokens,
  *   (a, b) -> (a cos - b sin, a sin + b cos)
  * with cos_table, sin_table [table_rows][rot_dim / 2] fp32 at the row's position; pairs are (i, i + rot_dim / 2), or
  * (2i, 2i + 1) when `interleaved`.  Results are rounded once to cache_type (F16 or BF16): q_out [tokens][q_heads][head_dim]
- * (may be q itself where it has that type and layout), k_cache and v_cache [num_pages][kv_heads][page_size][head_dim].
+ * (may be q itself where it has that type and layout), k_cache and v_cache [num_pages][kv_heads][page_size][head_dim], two arrays.
  * A row whose position is negative is left out altogether; one whose slot lies outside the cache gets its q_out and no
  * place in the cache.  A position at or above table_rows leaves the row out as well and records TB200_ERR_INVALID_ARG
  * (tb200_device_status).  Rows must not share a slot. */

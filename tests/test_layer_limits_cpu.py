@@ -2,7 +2,7 @@
 anything is launched (no GPU needed)."""
 import pytest
 
-from test_layer_cpu import INVALID, P, attention, norm, plan
+from test_layer_cpu import INVALID, P, append, attention, norm, plan
 
 
 @pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) - 8192, (1 << 31) - 1])
@@ -63,3 +63,10 @@ def test_plan_factory_refuses_outputs_over_other_arrays():
     for kw in (dict(kvLens=a["cachedLens"]), dict(cuNew=a["positions"]), dict(counts=a["freePages"]), dict(blockTable=a["positions"])):
         with pytest.raises(RuntimeError, match="one array"):
             B200.pagedPlan(**(a | kw))
+
+
+@pytest.mark.parametrize("kw", [dict(in_type=0), dict(in_type=2, q_stride=512), dict(in_type=1, cache_type=2), dict(in_type=2, k_cache=P + 4096, v_cache=P + 4096)])
+def test_append_refuses_outputs_over_what_is_still_read_or_written(lib, kw):
+    """q_out over a q of another type or row pitch, and one cache for keys and values: threads would overwrite each other."""
+    a = dict(q=P, q_out=P, k=P + 1024, v=P + 2048, k_cache=P + 4096, v_cache=P + 8192, cache_type=2) | kw
+    assert append(lib, **a) == INVALID

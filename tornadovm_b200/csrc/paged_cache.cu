@@ -393,6 +393,9 @@ extern "C" int tb200_rope_append(int tokens, int q_heads, int kv_heads, int head
     if (!aligned_to(q, b) || !aligned_to(k, b) || !aligned_to(v, b) || !aligned_to(q_out, 2) || !aligned_to(k_cache, 2) || !aligned_to(v_cache, 2) ||
         !aligned_to(cos_table, 4) || !aligned_to(sin_table, 4) || !aligned_to(positions, 4) || !aligned_to(slots, 8))
         return TB200_ERR_ALIGNMENT;
+    // a thread's results may replace what it has read itself, and nothing else
+    if (q_heads > 0 && q_out == q && (in_type != cache_type || (q_stride != (long long)q_heads * head_dim && tokens > 1))) return TB200_ERR_INVALID_ARG;
+    if (num_pages > 0 && k_cache == v_cache) return TB200_ERR_INVALID_ARG;
     int st;
     const DeviceInfo *di = device_info(&st);
     if (!di) return st;
