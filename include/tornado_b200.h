@@ -476,7 +476,8 @@ int tb200_rope_append(int tokens, int q_heads, int kv_heads, int head_dim, int i
  * places that a row does not see never reaches it, infinities and NaN included.
  * q, out and the caches [num_pages][kv_heads][page_size][head_dim] are of one type, F16 or BF16; head_dim is a multiple
  * of 8 up to 256, q_heads a multiple of kv_heads, scale > 0; the caches and out are 8-byte aligned.  out [tokens] rows
- * of q_heads * head_dim elements, out_stride apart; rows behind the last request are left as they were.
+ * of q_heads * head_dim elements, out_stride apart (it may be q itself where the strides agree); rows behind the last
+ * request are left as they were.
  * Scores, softmax and sums are fp32; probabilities are rounded to `type` for the product with V, and the result once (in
  * F16 a probability below 2^-21 of the largest one is off by up to 2^-32 of that).
  * max_new: an upper bound on the rows of one request (0: unknown); it only chooses kernels and never changes what is

@@ -9,7 +9,7 @@ import torch
 from harness import stream_ptr, sync_and_check
 from layer_util import BF16, F16, F32, HALF_STEP, HALF_TINY, Paged, fp8_values, from_bits, to_bits
 from oracle import layer as ol
-from test_layer_gpu import check_attention, run_attention, run_norm
+from test_layer_gpu import attention_args, attention_bufs, check_attention, run_attention, run_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -249,3 +249,18 @@ def test_plan_of_neighbouring_arrays_and_shared_lengths(lib):
     assert np.array_equal(take("table").reshape(n, width), want[0]) and np.array_equal(take("slots").view(np.int64), want[4])
     for k, w in (("cu", want[1]), ("kv", want[2]), ("positions", want[3]), ("counts", want[5])):
         assert np.array_equal(take(k), w), k
+
+
+# ---- attention: the result in the place of the queries --------------------------------------------------------------------
+@pytest.mark.parametrize("cached,new,page", [([3000, 40], [1, 1], 16), ([100, 30], [1, 1], 16), ([700, 20], [90, 150], 16), ([700, 20], [90, 150], 20), ([0, 0], [300, 5], 64)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_attention_in_place_of_its_queries(lib, cached, new, page, dim):
+    p = Paged(np.random.default_rng(dim), cached, new, 8, 2, dim, page, BF16, pad=2)
+    bufs = attention_bufs(p)
+    n = lib.tb200_paged_attention_workspace_bytes(p.tokens, 2, 8, 2, dim)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    q, used = bufs["q"].clone(), int(p.cu[-1])
+    for b in (bufs, bufs | {"q": q, "out": q}):
+        assert lib.tb200_paged_attention(*attention_args(p, b, ws, n, max_new=max(new)), stream_ptr()) == 0
+    sync_and_check(lib)
+    assert torch.equal(q[:used], bufs["out"][:used]) and torch.equal(q[used:], bufs["q"][used:])

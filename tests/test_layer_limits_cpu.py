@@ -70,3 +70,8 @@ def test_append_refuses_outputs_over_what_is_still_read_or_written(lib, kw):
     """q_out over a q of another type or row pitch, and one cache for keys and values: threads would overwrite each other."""
     a = dict(q=P, q_out=P, k=P + 1024, v=P + 2048, k_cache=P + 4096, v_cache=P + 8192, cache_type=2) | kw
     assert append(lib, **a) == INVALID
+
+
+def test_attention_refuses_an_out_over_q_at_another_pitch(lib):
+    assert attention(lib, q=P, out=P, q_stride=256, out_stride=264) == INVALID
+    assert attention(lib, q=P, out=P, q_stride=300, out_stride=256) == INVALID

@@ -504,6 +504,9 @@ extern "C" int tb200_paged_attention(int tokens, int requests, int max_new, int 
         return TB200_ERR_ALIGNMENT;
     if (!workspace || workspace_bytes < tb200_paged_attention_workspace_bytes(tokens, requests, q_heads, kv_heads, head_dim)) return TB200_ERR_WORKSPACE;
     if (!aligned_to(workspace, 16)) return TB200_ERR_ALIGNMENT;
+    // A block reads a tile's query rows before anybody stores that tile's results, and nobody else reads them: out may be q,
+    // but not at another pitch, where a row's results land on other rows.
+    if (out == q && out_stride != q_stride && tokens > 1) return TB200_ERR_INVALID_ARG;
     int st;
     const DeviceInfo *di = device_info(&st);
     if (!di) return st;
