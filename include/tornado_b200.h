@@ -414,7 +414,7 @@ int tb200_fp8gemm_f32(int m, int n, int k, int format, const uint8_t *a, const u
  * int8 blocks), the tables of a paged cache of keys and values, the write into it, and the attention that reads it.
  * No counterpart in the reference, whose models write these as JIT kernels.  All arrays are device arrays of the
  * calling thread's current CUDA context.  Pointers need the alignment of their element; 8 bytes (a payload behind
- * either array header) keeps vector loads, 16 bytes the widest ones. */
+ * either array header) keeps vector loads, 16 bytes the widest ones and the faster kernel of tb200_paged_attention. */
 enum tb200_type { TB200_TYPE_F32 = 0, TB200_TYPE_F16 = 1, TB200_TYPE_BF16 = 2 }; /* the values of tb200_gemm_out */
 enum tb200_quant_format { TB200_Q_INT8 = 0, TB200_Q_E4M3 = 1, TB200_Q_E5M2 = 2 };
 
@@ -458,8 +458,9 @@ int tb200_paged_plan(int requests, int page_size, int max_pages, int max_tokens,
  * (2i, 2i + 1) when `interleaved`.  Results are rounded once to cache_type (F16 or BF16): q_out [tokens][q_heads][head_dim]
  * (may be q itself where it has that type and layout), k_cache and v_cache [num_pages][kv_heads][page_size][head_dim], two arrays.
  * A row whose position is negative is left out altogether; one whose slot lies outside the cache gets its q_out and no
- * place in the cache.  A position at or above table_rows leaves the row out as well and records TB200_ERR_INVALID_ARG
- * (tb200_device_status).  Rows must not share a slot. */
+ * place in the cache.  With rot_dim > 0 a position at or above table_rows leaves the row out as well and records
+ * TB200_ERR_INVALID_ARG (tb200_device_status); with rot_dim 0 there are no tables, and positions only say which rows count.
+ * Rows must not share a slot. */
 int tb200_rope_append(int tokens, int q_heads, int kv_heads, int head_dim, int in_type, const void *q, const void *k, const void *v,
                       long long q_stride, long long k_stride, long long v_stride, const float *cos_table, const float *sin_table,
                       int table_rows, int rot_dim, int interleaved, const int32_t *positions, int cache_type, void *q_out,
@@ -481,7 +482,8 @@ int tb200_rope_append(int tokens, int q_heads, int kv_heads, int head_dim, int i
  * Scores, softmax and sums are fp32; probabilities are rounded to `type` for the product with V, and the result once (in
  * F16 a probability below 2^-21 of the largest one is off by up to 2^-32 of that).
  * max_new: an upper bound on the rows of one request (0: unknown); it only chooses kernels and never changes what is
- * computed.  The context of a request is split over the GPU and joined in a fixed order, so equal calls give equal
+ * computed.  More than 16 rows for one kv head (max_new * q_heads / kv_heads), and heads above 128, run on a kernel several
+ * times as fast where the caches are 16-byte aligned and page_size is a power of two from 8 on.  The context of a request is split over the GPU and joined in a fixed order, so equal calls give equal
  * results.  The workspace (16-byte aligned; tb200_paged_attention_workspace_bytes) needs no initialisation; two calls
  * that can run at the same time need one each.  requests, tokens * q_heads / kv_heads and max_pages * page_size <= 2^30. */
 size_t tb200_paged_attention_workspace_bytes(int tokens, int requests, int q_heads, int kv_heads, int head_dim);

@@ -438,7 +438,9 @@ static int attn_launch(AttnArgs a, int longest_rows, void *workspace, const Devi
     if (st) return st;
     int grid = min(di->sm_count, AT_MAX_SMS) * S::BLOCKS_PER_SM;
     // Short contexts: the search for a block's share and the join take longer than a whole item does.  Six requests of 157
-    // keys: 16.4 us split, 12.0 us whole; eight of 500 keys: 15.5 us split, 19.9 us whole.
+    // keys: 16.4 us split, 12.0 us whole; eight of 500 keys: 15.5 us split, 19.9 us whole.  (Measured on single tokens; the
+    // rule does not count row tiles, which a block takes one after another: a prompt of 250 tokens on 8 kv heads takes 42 us
+    // with pages of 20, on 8 blocks, and 25 us with pages of 16 on the other kernel.)
     const long long keys = min((long long)a.max_pages * a.page_size, a.window > 0 ? (long long)a.window + longest_rows / a.group : 1LL << 40);
     a.whole = keys <= AT_WHOLE_TILES * AT_KEYS && (long long)a.requests * a.kv_heads <= 0x3FFFFFFF;
     if (a.whole) {

@@ -24,7 +24,7 @@ struct AttnArgs {
     const void *q, *k_cache, *v_cache;
     const int32_t *cu_new, *kv_lens, *block_table;
     void *out;
-    float *parts;        // [grid][2][rows of a tile][pitch]: output, then maximum and sum
+    float *parts;        // [grid][2] parts of output, reference and sum: [rows of a tile][pitch] in attention.cu, [columns][rows] in attention_tc.cu
     int4 *joins;         // [grid]: item that the block begins and another one ends: (request, kv head, row tile, last block), x < 0: none
     long long q_stride, out_stride;
     float scale_log2;    // scale * log2(e): probabilities are powers of two

@@ -186,8 +186,10 @@ static int launch_plan(const PlanArgs &a, int threads, const DeviceInfo *di, cud
 // thread turns 16 elements of a head, eight and the eight that they pair with, as two wide loads and stores; threads
 // next to one another hold the rest of the head, so that a warp moves whole lines of the projection row and of the
 // cache (a head's row of a page is head_dim elements in one piece).  The angles of a row are read by all of its heads
-// and come out of L1.  8192 rows of 48 heads of 128 into slots in random order: 49 us, 0.64 of the copy rate; four heads
-// a thread, with the angles and the slot read once for all four, took 47 us and are not worth a second kernel.
+// and come out of L1.  8192 rows of 48 heads of 128 into slots in random order: 49.5 us, 0.63 of the copy rate: a thread's
+// source and angles are asked for behind its position, and its stores wait for the slot, three dependent latencies for 32
+// bytes in and out; and with interleaved pairs a thread's two 16-byte pieces lie side by side, so that an access of a warp
+// fills half of each sector it touches.  Four heads a thread, with the angles and the slot read once for all four, took 47 us.
 struct AppendArgs {
     const void *q, *k, *v;
     const float *cos_table, *sin_table;
