@@ -480,7 +480,8 @@ static int launch_norm(const NormArgs &a, int threads, const DeviceInfo *di, cud
         st = late ? ensure_kernel<rmsnorm_kernel<T, ALIGN, NV, STAGES, CAN_BE_LATE>, FLAGS>(di) : ensure_kernel<rmsnorm_kernel<T, ALIGN, NV, STAGES, false>, FLAGS>(di);
         if (st) return st;
         const long long resident = min((long long)a.rows, STAGES ? max(1LL, (long long)di->sm_count * (long long)(200 * 1024 / (smem + 1024))) : (long long)di->sm_count * (2048 / threads));
-        const int grid = (int)max(resident, (a.rows + NORM_ROWS - 1LL) / NORM_ROWS);
+        // whole waves of blocks of up to NORM_ROWS rows (20000 x 14336 bf16: 574 us in one wave, 669 us in 2.1 of them)
+        const int grid = (int)min((long long)a.rows, resident * ((a.rows + resident * NORM_ROWS - 1) / (resident * NORM_ROWS)));
         if (late) rmsnorm_kernel<T, ALIGN, NV, STAGES, CAN_BE_LATE><<<grid, threads, smem, s>>>(a);
         else rmsnorm_kernel<T, ALIGN, NV, STAGES, false><<<grid, threads, smem, s>>>(a);
     } else {
